@@ -441,6 +441,89 @@ int xl_softcap_argmax(const xl_greedy_params* p, void* cuda_stream);
 int32_t xl_softcap_argmax_noalloc_max_rows(void);
 int xl_softcap_argmax_noalloc(const xl_greedy_params* p, void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Sampling head: tokens[r] drawn from row r of soft-capped logits by a given uniform number.  (The reference decodes
+ * greedily only, xlstm/xlstm_large/generate.py:13-15; this is the sampling a serving loop needs in its place.)
+ *
+ * With y = soft cap of the logits, kept in 64-bit arithmetic, and w_j = exp((y_j - max y) / temperature), the tokens are
+ * taken in the order of descending logit, lower index first among equals, and
+ *   1. top_k    the first top_k are kept (<= 0: all);
+ *   2. top_p    of those, token j while the w in front of it sum to less than top_p of what step 1 kept (>= 1: all);
+ *   3. min_p    of those, tokens with w_j >= min_p (of the largest w, which is 1);
+ * the first token always stays.  The result is the first token whose running sum of kept w exceeds u times their total.
+ * A row with temperature <= 0 or NaN takes the token of xl_softcap_argmax.  NaN and -inf logits are never chosen (a row
+ * of nothing else gives token 0); with a +inf logit and no cap the +inf tokens share the row.  u outside [0, 1) is clamped.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct xl_sample_params {
+  const void* logits;       /* (rows, V) un-capped logits, dtype `dtype`, row stride row_stride elements */
+  int64_t* tokens;          /* out (rows) */
+  const float* u;           /* (rows) uniform numbers in [0, 1) */
+  const float* temperature_rows; const int32_t* top_k_rows; const float* top_p_rows; const float* min_p_rows;
+                            /* (rows) settings per row; NULL: the one below for every row */
+  int32_t rows, V;
+  int64_t row_stride;
+  float cap;                /* soft cap of the logits; 0: none */
+  float temperature; int32_t top_k; float top_p, min_p;
+  int32_t dtype;
+} xl_sample_params;
+
+/* Requires V <= 2^19.  Needs no scratch memory; calls may overlap. */
+int xl_softcap_sample(const xl_sample_params* p, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Top logits: of every row the k largest soft-capped logits in descending order (equal logits: lower index first) and
+ * lse = log sum_j exp(y_j / temperature) over the whole row -- what a teacher leaves behind for xl_distill_topk.
+ * The order is that of the un-capped logits (the cap is increasing); NaN comes last, behind -inf.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct xl_topk_params {
+  const void* logits;       /* (rows, V) un-capped logits, row stride row_stride elements */
+  float* values;            /* out (rows, k): y, not divided by the temperature */
+  int32_t* ids;             /* out (rows, k) */
+  float* lse;               /* out (rows) or NULL */
+  int32_t rows, V, k;       /* 1 <= k <= min(V, 1024), V <= 2^19 */
+  int64_t row_stride;
+  float cap;                /* 0: none */
+  float temperature;        /* > 0 */
+  int32_t dtype;
+} xl_topk_params;
+
+int xl_softcap_topk(const xl_topk_params* p, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Distillation from a teacher's top logits.  Row r has K teacher entries (values t_k: capped logits, ids); an id below 0 is
+ * an unused entry.  With z = soft_cap(logits) / T, q = softmax(z):
+ *   p_k = exp(t_k / T - L),  L = log sum over used entries of exp(t_k / T)        without teacher_lse (renormalised), or
+ *                            L = teacher_lse[r], and p_tail = max(0, 1 - sum p_k)  with it (the mass of all tokens not named);
+ *   loss = T^2 ( sum_k p_k (log p_k - log q[id_k]) + p_tail (log p_tail - log q_tail) ),  q_tail = sum of q over tokens not named;
+ *   dloss/dz_j = T^2 ( W q_j - sum_{k: id_k = j} p_k - p_tail q_j / q_tail [j not named] ),  W = sum p_k + p_tail.
+ * A row without a used entry (or, without teacher_lse, whose used entries are all -inf) has loss 0 and gradient 0.  Where
+ * every token is named p_tail counts as 0.  An id may be named twice.  An id >= V counts as unused and sets *status = 4.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct xl_distill_params {
+  const void* logits;       /* (rows, V) un-capped logits of the student, dtype `dtype`, row stride row_stride */
+  const float* values;      /* (rows, K) contiguous */
+  const void* ids;          /* (rows, K) contiguous, int32, or int64 with ids64 */
+  const float* teacher_lse; /* (rows) or NULL */
+  const float* weight;      /* factor of each row's gradient, element r * weight_stride (0: one for all); NULL: 1 */
+  float* loss;              /* out (rows) */
+  void* dlogits;            /* out (rows, V), dtype `dtype`, row stride dlogits_stride; must not overlap logits.
+                               xl_distill_topk: NULL for the losses alone */
+  float* stats;             /* (rows, 8) fp32, what the backward entry needs: out of xl_distill_topk (or NULL), in for
+                               xl_distill_topk_backward */
+  int32_t* status;          /* device word or NULL */
+  int32_t rows, V, K;       /* 1 <= K <= 1024, V <= 2^19 */
+  int32_t ids64;
+  int64_t row_stride, dlogits_stride, weight_stride;
+  float cap;                /* 0: none */
+  float temperature;        /* > 0 */
+  int32_t dtype;
+} xl_distill_params;
+
+/* Losses and, with dlogits, the gradient of sum_r weight[r] * loss[r]. */
+int xl_distill_topk(const xl_distill_params* p, void* cuda_stream);
+/* The gradient alone, behind xl_distill_topk on the same inputs (`loss` is not used). */
+int xl_distill_topk_backward(const xl_distill_params* p, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ EXPORTS = (
     "xl_softcap_argmax", "xl_softcap_argmax_scratch_bytes", "xl_swiglu",
     "xl_softcap_argmax_noalloc", "xl_softcap_argmax_noalloc_max_rows", "xl_peer_reduce_add_rmsnorm", "xl_headwise_proj", "xl_mlstm_decode_cell",
     "xl_slstm_backward", "xl_slstm_cache_bytes", "xl_slstm_weight_grads", "xl_slstm_weight_grads_scratch_bytes", "xl_rows_linear", "xl_rows_linear_ahead",
+    "xl_softcap_sample", "xl_softcap_topk", "xl_distill_topk", "xl_distill_topk_backward",
 )
 
 
@@ -152,6 +153,33 @@ class GreedyParams(C.Structure):
     ]
 
 
+class SampleParams(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("tokens", C.c_void_p), ("u", C.c_void_p),
+        ("temperature_rows", C.c_void_p), ("top_k_rows", C.c_void_p), ("top_p_rows", C.c_void_p), ("min_p_rows", C.c_void_p),
+        ("rows", C.c_int32), ("V", C.c_int32), ("row_stride", C.c_int64), ("cap", C.c_float),
+        ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float), ("dtype", C.c_int32),
+    ]
+
+
+class TopkParams(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("values", C.c_void_p), ("ids", C.c_void_p), ("lse", C.c_void_p),
+        ("rows", C.c_int32), ("V", C.c_int32), ("k", C.c_int32), ("row_stride", C.c_int64),
+        ("cap", C.c_float), ("temperature", C.c_float), ("dtype", C.c_int32),
+    ]
+
+
+class DistillParams(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("values", C.c_void_p), ("ids", C.c_void_p), ("teacher_lse", C.c_void_p), ("weight", C.c_void_p),
+        ("loss", C.c_void_p), ("dlogits", C.c_void_p), ("stats", C.c_void_p), ("status", C.c_void_p),
+        ("rows", C.c_int32), ("V", C.c_int32), ("K", C.c_int32), ("ids64", C.c_int32),
+        ("row_stride", C.c_int64), ("dlogits_stride", C.c_int64), ("weight_stride", C.c_int64),
+        ("cap", C.c_float), ("temperature", C.c_float), ("dtype", C.c_int32),
+    ]
+
+
 class PeerReduceParams(C.Structure):
     _fields_ = [
         ("partial", C.c_void_p), ("peer_recv", C.c_void_p), ("recv_local", C.c_void_p), ("peer_flags", C.c_void_p),
@@ -206,7 +234,9 @@ def lib() -> C.CDLL:
                             ("xl_softcap_argmax", GreedyParams), ("xl_swiglu", SwigluParams),
                             ("xl_softcap_argmax_noalloc", GreedyParams), ("xl_peer_reduce_add_rmsnorm", PeerReduceParams),
                             ("xl_slstm_backward", SlstmBwdParams), ("xl_slstm_weight_grads", SlstmWgradParams),
-                            ("xl_rows_linear", RowsLinearParams), ("xl_rows_linear_ahead", RowsLinearParams)):
+                            ("xl_rows_linear", RowsLinearParams), ("xl_rows_linear_ahead", RowsLinearParams),
+                            ("xl_softcap_sample", SampleParams), ("xl_softcap_topk", TopkParams),
+                            ("xl_distill_topk", DistillParams), ("xl_distill_topk_backward", DistillParams)):
             fn = getattr(l, name)
             fn.restype = C.c_int
             fn.argtypes = [C.POINTER(ptype), C.c_void_p]

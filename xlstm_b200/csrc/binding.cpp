@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 #include "../../include/xlstm_b200.h"
@@ -745,6 +746,217 @@ PyObject* softcap_argmax(PyObject*, PyObject* const* a, Py_ssize_t na) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------- along the vocabulary axis
+// The rows of un-capped logits (..., V) and what every entry checks about them.
+struct VocabRows {
+  Tensor x;
+  int64_t rows, V;
+  float cap;
+
+  VocabRows(const Tensor& logits, double cap_arg, const char* name) : cap((float)cap_arg) {
+    TORCH_CHECK_VALUE(known_dtype(logits), name, ": float32 or bfloat16 logits only");
+    TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, name, ": logits must be (..., V) with V > 0");
+    V = logits.size(-1);
+    x = as_rows(logits, V);
+    rows = x.size(0);
+    if (rows > 1 && x.stride(0) < V) x = x.contiguous();   // (expanded rows)
+    TORCH_CHECK_VALUE(rows <= INT32_MAX, name, ": too many rows");
+  }
+  int64_t stride() const { return rows > 1 ? x.stride(0) : V; }
+  // one value per row: any shape of that many elements
+  Tensor per_row(const Tensor& t, const char* name, const char* what) const {
+    TORCH_CHECK_VALUE(t.device() == x.device() && t.numel() == rows, name, ": ", what, " must have one entry per row of logits, on their device");
+    return t.reshape({rows}).contiguous();
+  }
+};
+// a cap: a positive number, or None for none
+double cap_arg(PyObject* o) {
+  if (o == Py_None) return 0.0;
+  const double v = double_arg(o);
+  TORCH_CHECK_VALUE(v > 0.0 && v < 3.0e38, "the soft cap must be positive (None: no cap)");
+  return v;
+}
+// a number, or a tensor of one per row; the number is checked against [lo, hi]
+struct Setting {
+  const Tensor* rows = nullptr;
+  double value = 0.0;
+  Setting(PyObject* o, const char* what, double lo, double hi) {
+    if (THPVariable_Check(o)) { rows = &THPVariable_Unpack(o); return; }
+    value = double_arg(o);
+    TORCH_CHECK_VALUE(value >= lo && value <= hi, "softcap_sample: ", what, " must lie in [", lo, ", ", hi, "], got ", value);
+  }
+};
+
+// (logits, cap or None, u, temperature, top_k, top_p, min_p: numbers or tensors of one per row) -> int64 tokens of shape logits.shape[:-1]
+PyObject* softcap_sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  want_args(na, 7);
+  const Tensor &logits = tensor_arg(a[0], "logits"), &u0 = tensor_arg(a[2], "u");
+  const double cap = cap_arg(a[1]);
+  const Setting temperature(a[3], "temperature", 0.0, 3.0e38), top_k(a[4], "top_k", 0.0, INT32_MAX), top_p(a[5], "top_p", 0.0, 1.0), min_p(a[6], "min_p", 0.0, 1.0);
+  Unlocked unlocked;
+  for (const Tensor* t : {&logits, &u0, temperature.rows, top_k.rows, top_p.rows, min_p.rows}) require_cuda(t);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const VocabRows r(logits, cap, "softcap_sample");
+  TORCH_CHECK_VALUE(top_k.value == std::floor(top_k.value), "softcap_sample: top_k must be a whole number");
+  TORCH_CHECK_VALUE(u0.scalar_type() == at::kFloat, "softcap_sample: u must be float32 (a number rounded up to 1 would leave [0, 1))");
+  xl_sample_params p = {};
+  const Tensor u = r.per_row(u0, "softcap_sample", "u");
+  Tensor keep[4];
+  auto floats = [&](const Setting& s, const char* what, Tensor& held) -> const float* {
+    if (!s.rows) return nullptr;
+    TORCH_CHECK_VALUE(s.rows->is_floating_point(), "softcap_sample: ", what, " must be a floating-point tensor");
+    held = as_float(r.per_row(*s.rows, "softcap_sample", what));
+    return held.const_data_ptr<float>();
+  };
+  p.temperature_rows = floats(temperature, "temperature", keep[0]);
+  p.top_p_rows = floats(top_p, "top_p", keep[1]);
+  p.min_p_rows = floats(min_p, "min_p", keep[2]);
+  if (top_k.rows) {
+    TORCH_CHECK_VALUE(top_k.rows->scalar_type() == at::kInt || top_k.rows->scalar_type() == at::kLong, "softcap_sample: top_k must be an int32 or int64 tensor");
+    keep[3] = r.per_row(*top_k.rows, "softcap_sample", "top_k");
+    if (keep[3].scalar_type() == at::kLong) keep[3] = keep[3].clamp(0, INT32_MAX).to(at::kInt);
+    p.top_k_rows = keep[3].const_data_ptr<int32_t>();
+  }
+  const Tensor out = empty_on(logits.sizes().slice(0, logits.dim() - 1), at::kLong, r.x);
+  int rc = XL_OK;
+  if (r.rows > 0) {
+    p.logits = r.x.data_ptr(); p.tokens = out.data_ptr<int64_t>(); p.u = u.const_data_ptr<float>();
+    p.rows = (int32_t)r.rows; p.V = (int32_t)r.V; p.row_stride = r.stride(); p.cap = r.cap;
+    p.temperature = (float)temperature.value; p.top_k = (int32_t)top_k.value; p.top_p = (float)top_p.value; p.min_p = (float)min_p.value;
+    p.dtype = dtype_code(r.x);
+    rc = xl_softcap_sample(&p, stream_of(r.x));
+  }
+  unlocked.lock();
+  check(rc, "xl_softcap_sample");
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (logits, cap or None, k, temperature) -> (values, ids, lse)
+PyObject* softcap_topk(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  want_args(na, 4);
+  const Tensor& logits = tensor_arg(a[0], "logits");
+  const double cap = cap_arg(a[1]), temperature = double_arg(a[3]);
+  const int64_t k = int_arg(a[2]);
+  Unlocked unlocked;
+  require_cuda(logits);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const VocabRows r(logits, cap, "softcap_topk");
+  TORCH_CHECK_VALUE(k >= 1 && k <= r.V, "softcap_topk: k must lie between 1 and the vocabulary size ", r.V, ", got ", k);
+  TORCH_CHECK_VALUE(temperature > 0.0 && temperature < 3.0e38, "softcap_topk: the temperature must be positive");
+  c10::SmallVector<int64_t, 5> sizes(logits.sizes().begin(), logits.sizes().end());
+  const Tensor lse = empty_on(at::IntArrayRef(sizes).slice(0, sizes.size() - 1), at::kFloat, r.x);
+  sizes.back() = k;
+  const Tensor values = empty_on(sizes, at::kFloat, r.x), ids = empty_on(sizes, at::kInt, r.x);
+  int rc = XL_OK;
+  if (r.rows > 0) {
+    xl_topk_params p = {};
+    p.logits = r.x.data_ptr(); p.values = values.data_ptr<float>(); p.ids = ids.data_ptr<int32_t>(); p.lse = lse.data_ptr<float>();
+    p.rows = (int32_t)r.rows; p.V = (int32_t)r.V; p.k = (int32_t)std::min<int64_t>(k, INT32_MAX); p.row_stride = r.stride(); p.cap = r.cap;
+    p.temperature = (float)temperature; p.dtype = dtype_code(r.x);
+    rc = xl_softcap_topk(&p, stream_of(r.x));
+  }
+  unlocked.lock();
+  check(rc, "xl_softcap_topk");
+  return pack({values, ids, lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// What the loss and its gradient share.  The members keep converted tensors alive until the launch.
+struct DistillArgs {
+  VocabRows r;
+  Tensor values, ids, lse, weight;
+  xl_distill_params p = {};
+
+  DistillArgs(const Tensor& logits, const Tensor& values0, const Tensor& ids0, const Tensor* weight0, double cap, double temperature, const Tensor* lse0)
+      : r(logits, cap, "distill_topk") {
+    const int64_t K = values0.dim() ? values0.size(-1) : 0;
+    TORCH_CHECK_VALUE(values0.dim() == logits.dim() && values0.sizes() == ids0.sizes() && K > 0 &&
+                          values0.sizes().slice(0, values0.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+                      "distill_topk: values and ids must be (..., K) with the leading dimensions of logits");
+    TORCH_CHECK_VALUE(values0.is_floating_point() && (ids0.scalar_type() == at::kInt || ids0.scalar_type() == at::kLong),
+                      "distill_topk: floating-point values, int32 or int64 ids");
+    TORCH_CHECK_VALUE(values0.device() == logits.device() && ids0.device() == logits.device(), "distill_topk: values and ids must be on the device of logits");
+    TORCH_CHECK_VALUE(temperature > 0.0 && temperature < 3.0e38, "distill_topk: the temperature must be positive");
+    values = float_contig(values0);
+    ids = ids0.contiguous();
+    p.logits = r.x.data_ptr(); p.values = values.const_data_ptr<float>(); p.ids = ids.data_ptr(); p.ids64 = ids.scalar_type() == at::kLong;
+    if (lse0) {
+      lse = as_float(r.per_row(*lse0, "distill_topk", "teacher_lse"));
+      p.teacher_lse = lse.const_data_ptr<float>();
+    }
+    if (weight0) {   // (the gradient of a sum or a mean arrives expanded: one number for all rows)
+      TORCH_CHECK_VALUE(weight0->device() == logits.device() && weight0->numel() == r.rows && weight0->is_floating_point(),
+                        "distill_topk: weights must have one entry per row of logits, on their device");
+      bool one = true;
+      for (int64_t d = 0; d < weight0->dim(); ++d) one = one && (weight0->stride(d) == 0 || weight0->size(d) == 1);
+      weight = as_float(one || weight0->dim() == 1 ? *weight0 : weight0->reshape({r.rows}));
+      p.weight = weight.const_data_ptr<float>();
+      p.weight_stride = one ? 0 : weight.stride(0);
+    }
+    p.rows = (int32_t)r.rows; p.V = (int32_t)r.V; p.K = (int32_t)std::min<int64_t>(K, INT32_MAX);
+    p.row_stride = r.stride(); p.dlogits_stride = r.V;
+    p.cap = r.cap; p.temperature = (float)temperature; p.dtype = dtype_code(r.x);
+  }
+};
+
+// (logits, values, ids, weight or None, cap or None, temperature, teacher_lse or None, mode) -> loss | (loss, stats) | (loss, dlogits)
+// for mode 0, 1 (stats: what distill_topk_backward needs), 2 (gradient of the weighted sum of the losses)
+PyObject* distill_topk(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  want_args(na, 8);
+  const Tensor &logits = tensor_arg(a[0], "logits"), &values = tensor_arg(a[1], "values"), &ids = tensor_arg(a[2], "ids");
+  const Tensor *weight = optional_arg(a[3], "weight"), *lse = optional_arg(a[6], "teacher_lse");
+  const double cap = cap_arg(a[4]), temperature = double_arg(a[5]);
+  const int64_t mode = int_arg(a[7]);
+  Unlocked unlocked;
+  for (const Tensor* t : {&logits, &values, &ids, weight, lse}) require_cuda(t);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  DistillArgs d(logits, values, ids, weight, cap, temperature, lse);
+  const Tensor loss = empty_on(logits.sizes().slice(0, logits.dim() - 1), at::kFloat, logits);
+  Tensor extra;
+  d.p.loss = loss.data_ptr<float>();
+  if (mode == 1) {
+    extra = empty_on({d.r.rows, 8}, at::kFloat, logits);
+    d.p.stats = extra.data_ptr<float>();
+  } else if (mode == 2) {
+    extra = empty_on(logits.sizes(), logits.scalar_type(), logits);
+    d.p.dlogits = extra.data_ptr();
+  }
+  d.p.status = status_ptr(logits);
+  const int rc = d.r.rows > 0 ? xl_distill_topk(&d.p, stream_of(logits)) : XL_OK;
+  unlocked.lock();
+  check(rc, "xl_distill_topk");
+  return mode ? pack({loss, extra}) : THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
+// (logits, values, ids, dloss, cap or None, temperature, teacher_lse or None, stats) -> dlogits
+PyObject* distill_topk_backward(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  want_args(na, 8);
+  const Tensor &logits = tensor_arg(a[0], "logits"), &values = tensor_arg(a[1], "values"), &ids = tensor_arg(a[2], "ids"), &dloss = tensor_arg(a[3], "dloss");
+  const Tensor* lse = optional_arg(a[6], "teacher_lse");
+  const Tensor& stats = tensor_arg(a[7], "stats");
+  const double cap = cap_arg(a[4]), temperature = double_arg(a[5]);
+  Unlocked unlocked;
+  for (const Tensor* t : {&logits, &values, &ids, &dloss, lse, &stats}) require_cuda(t);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  DistillArgs d(logits, values, ids, &dloss, cap, temperature, lse);
+  TORCH_CHECK_VALUE(stats.sizes() == at::IntArrayRef({d.r.rows, 8}) && stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.device() == logits.device(),
+                    "stats do not belong to a forward call of these sizes");
+  const Tensor dx = empty_on(logits.sizes(), logits.scalar_type(), logits);
+  d.p.dlogits = dx.data_ptr(); d.p.stats = stats.data_ptr<float>();
+  d.p.status = status_ptr(logits);
+  const int rc = d.r.rows > 0 ? xl_distill_topk_backward(&d.p, stream_of(logits)) : XL_OK;
+  unlocked.lock();
+  check(rc, "xl_distill_topk_backward");
+  return THPVariable_Wrap(dx);
+  END_HANDLE_TH_ERRORS
+}
+
 // ---------------------------------------------------------------------------------------------- host-side vectors
 // A Python sequence of integers, or a tensor on the host that is one.
 std::vector<int64_t> host_integers(PyObject* o) {
@@ -849,6 +1061,7 @@ PyObject* status_word(PyObject*, PyObject* index) {
 PyMethodDef methods[] = {
     XL_FAST(mlstm_sequence), XL_FAST(mlstm_step), XL_FAST(mlstm_decode_cell), XL_FAST(slstm_forward), XL_FAST(slstm_backward), XL_FAST(slstm_weight_grads), XL_FAST(rows_linear),
     XL_FAST(add_rmsnorm), XL_FAST(headnorm_gate), XL_FAST(soft_cap), XL_FAST(causal_conv1d), XL_FAST(headwise_proj), XL_FAST(softcap_argmax),
+    XL_FAST(softcap_sample), XL_FAST(softcap_topk), XL_FAST(distill_topk), XL_FAST(distill_topk_backward),
     XL_FAST(document_offsets), XL_FAST(slot_vector),
     {"swiglu", swiglu, METH_O, nullptr}, {"status_word", status_word, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of xlstm_b200.ops.", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -10,6 +10,7 @@
 // candidate in SCRATCH memory and takes a ticket from the row's counter there; the block that draws the last ticket
 // reduces the row's candidates, writes the token and puts the counter back to zero for the next call.
 #include "common.cuh"
+#include "vocab_row.cuh"
 
 namespace xl {
 
@@ -28,12 +29,6 @@ struct GhRow {
 };
 
 __device__ __forceinline__ bool gh_better(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
-
-template <typename T> __device__ __forceinline__ float gh_capped(T x, float cap) {
-  const T q = from_float<T>(to_float(x) / cap);
-  const T t = from_float<T>(tanhf(to_float(q)));
-  return to_float(from_float<T>(cap * to_float(t)));
-}
 
 template <typename T>
 __global__ void __launch_bounds__(GH_THREADS) greedy_head_kernel(const xl_greedy_params p, GhRow* __restrict__ scratch) {
@@ -56,7 +51,7 @@ __global__ void __launch_bounds__(GH_THREADS) greedy_head_kernel(const xl_greedy
       *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(x + (long long)v * V16);
 #pragma unroll
       for (int i = 0; i < V16; ++i) {
-        const float y = gh_capped<T>(e[i], p.cap);
+        const float y = capped_rounded<T>(e[i], p.cap);
         if (gh_better(y, v * V16 + i, bv, bi)) { bv = y; bi = v * V16 + i; }
       }
     }
@@ -64,7 +59,7 @@ __global__ void __launch_bounds__(GH_THREADS) greedy_head_kernel(const xl_greedy
     const int per = (p.V + parts - 1) / parts;
     const int v0 = part * per, v1 = min(p.V, v0 + per);
     for (int v = v0 + tid; v < v1; v += GH_THREADS) {
-      const float y = gh_capped<T>(x[v], p.cap);
+      const float y = capped_rounded<T>(x[v], p.cap);
       if (gh_better(y, v, bv, bi)) { bv = y; bi = v; }
     }
   }

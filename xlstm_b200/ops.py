@@ -352,3 +352,69 @@ def softcap_argmax(logits, cap: float):
     contiguous rows; returns int64 of shape ``logits.shape[:-1]``.  The kernel's scratch area is allocated once per
     device (and grown when more rows come) and shared by all calls on that device's streams in issue order."""
     return native().softcap_argmax(logits, cap)
+
+
+def softcap_sample(logits, cap: Optional[float], u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Sampled tokens of un-capped logits, from given uniform numbers: int64 of shape ``logits.shape[:-1]``.
+
+    ``logits`` (..., V), ``cap`` the soft cap of the model's logits (None: none), ``u`` one float32 number in [0, 1) per
+    row.  ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are numbers, or CUDA tensors of one per row (numbers are
+    checked, tensors are not looked at: values outside their range act like the end of it).  They are applied in that
+    order: the weights are ``exp((y - max y) / temperature)`` of the capped logits y; the ``top_k`` largest logits stay (0:
+    all; of equal ones the lower indices); of those, a token stays while the tokens in front of it hold less than
+    ``top_p`` of their mass; of those, tokens of at least ``min_p`` times the largest weight; always the first.  The token is
+    the one where the running sum, in order of descending logits, passes ``u`` times the total (``u = 0``: the largest).
+
+    A row with temperature 0 takes the token of :func:`softcap_argmax` -- its ties are those of the capped logits rounded to
+    the dtype, where sampling keeps the cap in 64-bit arithmetic.  NaN and -inf logits (masked tokens) are never chosen;
+    a row of nothing else gives token 0."""
+    return native().softcap_sample(logits, cap, u, temperature, top_k, top_p, min_p)
+
+
+def softcap_topk(logits, cap: Optional[float], k: int, temperature: float = 1.0):
+    """The ``k`` largest soft-capped logits of every row and the row's log-sum-exp: what a teacher leaves for
+    :func:`distill_topk`.  Returns ``values`` (..., k) float32 (capped, not divided by the temperature, descending; equal
+    logits: lower index first; NaN last), ``ids`` (..., k) int32 and ``lse`` (...) float32, the log of the sum of
+    ``exp(y / temperature)`` over all V.  ``k`` up to 1024."""
+    return native().softcap_topk(logits, cap, k, temperature)
+
+
+class DistillFunction(torch.autograd.Function):
+    """``distill_topk`` with a backward pass; the logits are read once in each direction."""
+
+    @staticmethod
+    def forward(ctx, logits, values, ids, cap, temperature, teacher_lse):
+        loss, stats = native().distill_topk(logits, values, ids, None, cap, temperature, teacher_lse, 1)
+        ctx.save_for_backward(logits, values, ids, teacher_lse, stats)
+        ctx.cap, ctx.temperature = cap, temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        logits, values, ids, teacher_lse, stats = ctx.saved_tensors
+        return native().distill_topk_backward(logits, values, ids, dloss, ctx.cap, ctx.temperature, teacher_lse, stats), None, None, None, None, None
+
+
+def distill_topk(logits, values, ids, cap: Optional[float] = None, temperature: float = 1.0, teacher_lse=None):
+    """Distillation loss of every row against a teacher's top logits, differentiable in ``logits``.
+
+    ``logits`` (..., V) un-capped, of the student; ``values`` and ``ids`` (..., K) as :func:`softcap_topk` gives them (an id
+    below 0: unused entry; K up to 1024).  With T the temperature, q the softmax of the student's capped logits over T and p
+    the softmax of the entries over T, the loss is ``T**2 * sum p (log p - log q)`` (float32, shape ``logits.shape[:-1]``).
+    With ``teacher_lse`` -- the teacher's log-sum-exp over its whole vocabulary at the same temperature -- p are the
+    teacher's own probabilities, and what they leave to 1 stands against the student's mass on all tokens not named.
+
+    A row without a used entry costs nothing and has gradient 0 (padding).  A token named twice counts with both its
+    entries.  Ids beyond V count as unused and are reported by :func:`check_device_status`.  The teacher's tensors get no
+    gradient."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return DistillFunction.apply(logits, values, ids, cap, temperature, teacher_lse)
+    return native().distill_topk(logits, values, ids, None, cap, temperature, teacher_lse, 0)
+
+
+def distill_topk_grad(logits, values, ids, weight=None, cap: Optional[float] = None, temperature: float = 1.0, teacher_lse=None):
+    """:func:`distill_topk` and the gradient of ``sum(weight * loss)`` in one call: ``(loss, dlogits)``, not recorded by
+    autograd.  For a training step that knows the weight of every row beforehand (``weight`` (...), None: 1), typically
+    behind the head of a piece of the batch: ``logits.backward(dlogits)``.  The logits come from memory once for both."""
+    return native().distill_topk(logits, values, ids, weight, cap, temperature, teacher_lse, 2)
