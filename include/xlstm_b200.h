@@ -462,7 +462,7 @@ typedef struct xl_sample_params {
                             /* (rows) settings per row; NULL: the one below for every row */
   int32_t rows, V;
   int64_t row_stride;
-  float cap;                /* soft cap of the logits; 0: none */
+  float cap;                /* soft cap of the logits, 1e-6 .. 1e6; 0: none */
   float temperature; int32_t top_k; float top_p, min_p;
   int32_t dtype;
 } xl_sample_params;
@@ -482,8 +482,8 @@ typedef struct xl_topk_params {
   float* lse;               /* out (rows) or NULL */
   int32_t rows, V, k;       /* 1 <= k <= min(V, 1024), V <= 2^19 */
   int64_t row_stride;
-  float cap;                /* 0: none */
-  float temperature;        /* > 0 */
+  float cap;                /* 1e-6 .. 1e6; 0: none */
+  float temperature;        /* 1e-4 .. 1e6 */
   int32_t dtype;
 } xl_topk_params;
 
@@ -508,14 +508,14 @@ typedef struct xl_distill_params {
   float* loss;              /* out (rows) */
   void* dlogits;            /* out (rows, V), dtype `dtype`, row stride dlogits_stride; must not overlap logits.
                                xl_distill_topk: NULL for the losses alone */
-  float* stats;             /* (rows, 8) fp32, what the backward entry needs: out of xl_distill_topk (or NULL), in for
+  float* stats;             /* (rows, 8) fp32, 8-byte aligned, what the backward entry needs: out of xl_distill_topk (or NULL), in for
                                xl_distill_topk_backward */
   int32_t* status;          /* device word or NULL */
   int32_t rows, V, K;       /* 1 <= K <= 1024, V <= 2^19 */
   int32_t ids64;
   int64_t row_stride, dlogits_stride, weight_stride;
-  float cap;                /* 0: none */
-  float temperature;        /* > 0 */
+  float cap;                /* 1e-6 .. 1e6; 0: none */
+  float temperature;        /* 1e-4 .. 1e6 */
   int32_t dtype;
 } xl_distill_params;
 

@@ -773,7 +773,7 @@ struct VocabRows {
 double cap_arg(PyObject* o) {
   if (o == Py_None) return 0.0;
   const double v = double_arg(o);
-  TORCH_CHECK_VALUE(v > 0.0 && v < 3.0e38, "the soft cap must be positive (None: no cap)");
+  TORCH_CHECK_VALUE(v >= 1e-6 && v <= 1e6, "the soft cap must lie in [1e-6, 1e6] (None: no cap)");
   return v;
 }
 // a number, or a tensor of one per row; the number is checked against [lo, hi]
@@ -845,7 +845,7 @@ PyObject* softcap_topk(PyObject*, PyObject* const* a, Py_ssize_t na) {
   const c10::cuda::CUDAGuard guard(logits.device());
   const VocabRows r(logits, cap, "softcap_topk");
   TORCH_CHECK_VALUE(k >= 1 && k <= r.V, "softcap_topk: k must lie between 1 and the vocabulary size ", r.V, ", got ", k);
-  TORCH_CHECK_VALUE(temperature > 0.0 && temperature < 3.0e38, "softcap_topk: the temperature must be positive");
+  TORCH_CHECK_VALUE(temperature >= 1e-4 && temperature <= 1e6, "softcap_topk: the temperature must lie in [1e-4, 1e6]");
   c10::SmallVector<int64_t, 5> sizes(logits.sizes().begin(), logits.sizes().end());
   const Tensor lse = empty_on(at::IntArrayRef(sizes).slice(0, sizes.size() - 1), at::kFloat, r.x);
   sizes.back() = k;
@@ -879,7 +879,7 @@ struct DistillArgs {
     TORCH_CHECK_VALUE(values0.is_floating_point() && (ids0.scalar_type() == at::kInt || ids0.scalar_type() == at::kLong),
                       "distill_topk: floating-point values, int32 or int64 ids");
     TORCH_CHECK_VALUE(values0.device() == logits.device() && ids0.device() == logits.device(), "distill_topk: values and ids must be on the device of logits");
-    TORCH_CHECK_VALUE(temperature > 0.0 && temperature < 3.0e38, "distill_topk: the temperature must be positive");
+    TORCH_CHECK_VALUE(temperature >= 1e-4 && temperature <= 1e6, "distill_topk: the temperature must lie in [1e-4, 1e6]");
     values = float_contig(values0);
     ids = ids0.contiguous();
     p.logits = r.x.data_ptr(); p.values = values.const_data_ptr<float>(); p.ids = ids.data_ptr(); p.ids64 = ids.scalar_type() == at::kLong;

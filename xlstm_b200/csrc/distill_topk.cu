@@ -13,142 +13,319 @@
 namespace xl {
 
 constexpr int DT_THREADS = 256, DT_WARPS = DT_THREADS / 32;
-// what a row leaves for its gradient
-enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_TEACHER = 4, ST_LIVE = 5 };
+constexpr double DT_LN2 = 0.69314718055994530942;
+// what a row leaves for its gradient; the last two places hold a double
+enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_LIVE = 4, ST_TEACHER = 6 };
 
 struct DtShared {
-  int id[TOPK_MAX];          // -1: unused
-  float p[TOPK_MAX], z[TOPK_MAX];
-  double wd[DT_WARPS];
-  float wf[DT_WARPS];
-  int wi[DT_WARPS];
+  double wd[2][DT_WARPS];
+  float wf[2][DT_WARPS], from[3][8];   // from: of the row's blocks; a place is written once a launch
+  int wi[2][DT_WARPS];
+  float lR, l, B, W, pscale;
 };
-
-struct DtTeacher {
-  double L;        // subtracted from t / T
-  double psum;
-  bool live;       // the row counts: an entry is used and, without the teacher's own sum, has mass
+// behind it: K entries -- t / T, id (-1: unused), z of the student there, e^(t / T - shift) -- and a bit per token of the slice
+struct DtEntries {
+  double* t;
+  int* id;
+  float *z, *e;
+  unsigned int* bits;
+  __device__ __forceinline__ DtEntries(unsigned char* m, int K) {
+    t = reinterpret_cast<double*>(m);
+    id = reinterpret_cast<int*>(t + K);
+    z = reinterpret_cast<float*>(id + K);
+    e = z + K;
+    bits = reinterpret_cast<unsigned int*>(e + K);
+  }
 };
-
-__device__ __forceinline__ float dt_tanh(float x, float cap) { return tanhf(x / cap); }
-
-// ids and probabilities of the teacher entries of a row into shared memory
-__device__ DtTeacher dt_teacher(DtShared& s, const xl_distill_params& p, long long row) {
-  const double invT = 1.0 / (double)p.temperature;
-  const float* val = p.values + row * p.K;
-  const bool given = p.teacher_lse != nullptr;
-  double m = -INFINITY;
-  int any = 0;
-  for (int k = threadIdx.x; k < p.K; k += DT_THREADS) {
-    const long long id = p.ids64 ? static_cast<const int64_t*>(p.ids)[row * p.K + k] : (long long)static_cast<const int32_t*>(p.ids)[row * p.K + k];
-    const bool used = id >= 0 && id < p.V;
-    if (id >= p.V && p.status) atomicExch(p.status, 4);
-    s.id[k] = used ? (int)id : -1;
-    any |= used;
-    if (used) m = fmax(m, (double)val[k] * invT);
-    if (used && val[k] != val[k]) m = val[k];
-  }
-  // (NaN has to survive the maximum)
-  m = block_reduce<DT_WARPS>(m, [](double a, double b) { return a != a ? a : b != b ? b : fmax(a, b); }, s.wd);
-  DtTeacher t;
-  any = block_reduce<DT_WARPS>(any, OpMax(), s.wi);
-  t.live = any && (given || m != -INFINITY);
-  t.L = 0.0;
-  if (t.live && !given) {
-    double sum = 0.0;
-    for (int k = threadIdx.x; k < p.K; k += DT_THREADS)
-      if (s.id[k] >= 0) sum += exp((double)val[k] * invT - m);
-    sum = block_reduce<DT_WARPS>(sum, OpSum(), s.wd);
-    t.L = m + log(sum);
-  } else if (given) {
-    t.L = (double)p.teacher_lse[row];
-  }
-  double psum = 0.0;
-  for (int k = threadIdx.x; k < p.K; k += DT_THREADS) {
-    const double pk = s.id[k] >= 0 && t.live ? exp((double)val[k] * invT - t.L) : 0.0;
-    s.p[k] = (float)pk;
-    psum += pk;
-  }
-  t.psum = block_reduce<DT_WARPS>(psum, OpSum(), s.wd);
-  return t;
+static size_t dt_smem(int K, int V, int N, int blocks) {
+  const size_t vectors = (size_t)V / N, places = ((vectors + blocks - 1) / blocks + 3) * N;
+  return (size_t)K * 20 + (places + 31) / 32 * 4 + 4;
 }
 
-template <typename T, bool LOSS, bool GRAD> __global__ void __launch_bounds__(DT_THREADS) distill_kernel(const xl_distill_params p) {
-  extern __shared__ __align__(16) unsigned int named[];   // a bit per token
+// one value of every block of the row's cluster, in rank order, combined by `f`
+template <typename F> __device__ __forceinline__ float dt_exchange(float v, float* from, int rank, int blocks, F f) {
+  if (threadIdx.x < blocks) st_cluster_f32(mapa_u32(smem_u32(from + rank), threadIdx.x), v);
+  cluster_sync_all();
+  v = from[0];
+  for (int r = 1; r < blocks; ++r) v = f(v, from[r]);
+  return v;
+}
+
+// Bound: with a cap |z| <= a, so that sums of 2^z need no maximum in front: 2^a * 2^19 and 2^-a stay normal numbers.
+constexpr float DT_BOUND = 100.f;
+
+template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD>
+__global__ void __launch_bounds__(DT_THREADS) distill_kernel(const xl_distill_params p, const int blocks) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ DtShared s;
-  const int tid = threadIdx.x, V = p.V, K = p.K;
-  const long long row = blockIdx.x;
+  constexpr int N = Vec16<T>::N;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, K = p.K;
+  const int rank = blocks > 1 ? (int)cluster_ctarank() : 0;
+  const long long row = blockIdx.x / blocks;
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
-  const float invT = 1.f / p.temperature, cap = p.cap;
+  const RowSlice<T> slice(x, V, rank, blocks);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + slice.head);
+  const CappedZ<CAP> Z(p.cap, p.temperature);
+  const DtEntries en(dynamic, K);
+  const bool given = p.teacher_lse != nullptr;
   float* st = p.stats ? p.stats + row * 8 : nullptr;
-  auto z_of = [&](float v) { return (cap > 0.f ? cap * dt_tanh(v, cap) : v) * invT; };
-  auto in_top = [&](int j) { return (named[j >> 5] >> (j & 31)) & 1u; };
+  const unsigned char* bytes = reinterpret_cast<const unsigned char*>(en.bits);
+  auto flags = [&](int v) -> unsigned int {   // bits of the vector's elements
+    const int o = N * (v + 1) - slice.first;
+    return N == 8 ? bytes[o >> 3] : (unsigned int)(bytes[o >> 3] >> (o & 4)) & 15u;
+  };
+  auto flag = [&](int j) -> bool {
+    const int o = slice.place(j) - slice.first;
+    return (en.bits[o >> 5] >> (o & 31)) & 1u;
+  };
 
-  const DtTeacher t = dt_teacher(s, p, row);
-  for (int w = tid; w < (V + 31) / 32; w += DT_THREADS) named[w] = 0u;
+  // (shared memory of another block may be written once that block runs: the other half of this barrier is in front of the first exchange)
+  if (LOSS && blocks > 1) cluster_arrive();
+  // the teacher's entries, the student's logits there, and the bits of the tokens named
+  for (int w = tid; w < (slice.end - slice.first + 31) / 32; w += DT_THREADS) en.bits[w] = 0u;
   __syncthreads();
-  int count = 0;   // of tokens named
-  for (int k = tid; k < K; k += DT_THREADS)
-    if (s.id[k] >= 0) count += !((atomicOr(&named[s.id[k] >> 5], 1u << (s.id[k] & 31)) >> (s.id[k] & 31)) & 1u);
-  count = block_reduce<DT_WARPS>(count, OpSum(), s.wi);   // (and the bits are there)
+  const double invT = 1.0 / (double)p.temperature;
+  double m = -INFINITY;   // of t / T
+  float mS = -INFINITY;
+  int any = 0, twice = 0, count = 0;
+  for (int k = tid; k < K; k += DT_THREADS) {
+    const long long at = row * K + k, id = p.ids64 ? static_cast<const int64_t*>(p.ids)[at] : (long long)static_cast<const int32_t*>(p.ids)[at];
+    const bool used = id >= 0 && id < V;
+    if (id >= V && p.status) atomicExch(p.status, 4);
+    en.id[k] = used ? (int)id : -1;
+    en.z[k] = 0.f;
+    if (!used) continue;
+    const double t = (double)p.values[at] * invT;
+    en.t[k] = t;
+    any = 1;
+    m = t != t || m != m ? t + m : fmax(m, t);   // (NaN survives)
+    en.z[k] = Z(to_float(x[id]));
+    mS = fmaxf(mS, en.z[k]);
+    const int o = slice.place((int)id) - slice.first;
+    if (o >= 0 && o < slice.end - slice.first) {
+      const int old = (atomicOr(&en.bits[o >> 5], 1u << (o & 31)) >> (o & 31)) & 1u;
+      twice |= old;
+      count += 1 - old;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double om = __shfl_xor_sync(0xffffffffu, m, o);
+    m = om != om || m != m ? om + m : fmax(m, om);
+    mS = fmaxf(mS, __shfl_xor_sync(0xffffffffu, mS, o));
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  any = __any_sync(0xffffffffu, any) | (__any_sync(0xffffffffu, twice) << 1);
+  if (lane == 0) { s.wd[0][warp] = m; s.wf[0][warp] = mS; s.wi[0][warp] = any; s.wi[1][warp] = count; }
+  __syncthreads();   // (the bits are there, too)
+  any = 0; count = 0;
+#pragma unroll
+  for (int w = 0; w < DT_WARPS; ++w) {
+    m = w == 0 ? s.wd[0][0] : s.wd[0][w] != s.wd[0][w] || m != m ? s.wd[0][w] + m : fmax(m, s.wd[0][w]);
+    mS = w == 0 ? s.wf[0][0] : fmaxf(mS, s.wf[0][w]);
+    any |= s.wi[0][w];
+    count += s.wi[1][w];
+  }
+  const bool again = any & 2, live = (any & 1) && (given || m != -INFINITY);
+  double L = 0.0;   // shift of the teacher's exponents; with its own sum, or in the backward pass, the right one from the start
+  if (live) {
+    if (!LOSS) L = *reinterpret_cast<const double*>(st + ST_TEACHER);
+    else L = given ? (double)p.teacher_lse[row] : m;
+  }
 
-  float lR, l, B, W;
   if (LOSS) {
-    float mR = -INFINITY, mS = -INFINITY;
-    for (int j = tid; j < V; j += DT_THREADS) {
-      const float z = z_of(to_float(x[j]));
-      if (in_top(j)) mS = fmaxf(mS, z);
-      else mR = fmaxf(mR, z);
+    if (blocks > 1) cluster_wait();
+    float mR = 0.f;
+    if (!BOUNDED) {
+      float xm = -INFINITY;
+      for (int v = slice.v0 + tid; v < slice.v1; v += DT_THREADS) {
+        Vec16<T> a;
+        a.set(__ldg(xv + v));
+        const unsigned int f = flags(v);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float x0, x1;
+          f2_unpack(a.p[i], x0, x1);
+          if (!(f >> (2 * i) & 1u)) xm = fmaxf(xm, x0);
+          if (!(f >> (2 * i + 1) & 1u)) xm = fmaxf(xm, x1);
+        }
+      }
+      for (int i = tid; i < slice.n_single(rank, blocks); i += DT_THREADS) {
+        const int j = slice.single(i, rank);
+        if (!flag(j)) xm = fmaxf(xm, to_float(x[j]));
+      }
+      xm = block_reduce<DT_WARPS>(xm, OpMax(), s.wf[1]);
+      if (blocks > 1) xm = dt_exchange(xm, s.from[2], rank, blocks, OpMax());
+      mR = xm == -INFINITY ? 0.f : Z(xm);
+      mS = mS == -INFINITY ? 0.f : mS;
+    } else {
+      mS = 0.f;
     }
-    mR = block_reduce<DT_WARPS>(mR, OpMax(), s.wf);
-    mS = block_reduce<DT_WARPS>(mS, OpMax(), s.wf);
-    const float m = fmaxf(mR, mS);
+    // both sums over the slice
     float sR = 0.f, sS = 0.f;
-    const float aR = mR == -INFINITY ? 0.f : mR, aS = mS == -INFINITY ? 0.f : mS;
-    for (int j = tid; j < V; j += DT_THREADS) {
-      const float z = z_of(to_float(x[j]));
-      if (in_top(j)) sS += expf(z - aS);
-      else sR += expf(z - aR);
+    f32x2 acc[2] = {0ull, 0ull};
+    const f32x2 shift = f2_dup(-mR);
+    auto sum = [&](const uint4& u, int v) {
+      Vec16<T> a;
+      a.set(u);
+      f32x2 z[N / 2];
+      Z.template of<T>(a, z);
+      const unsigned int f = flags(v);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        float z0, z1;
+        f2_unpack(BOUNDED ? z[i] : f2_add(z[i], shift), z0, z1);
+        float e0 = exp2_approx(z0), e1 = exp2_approx(z1);
+        if (f) {   // (rare: K of V tokens)
+          f2_unpack(z[i], z0, z1);
+          if (f >> (2 * i) & 1u) { sS += exp2_approx(z0 - mS); e0 = 0.f; }
+          if (f >> (2 * i + 1) & 1u) { sS += exp2_approx(z1 - mS); e1 = 0.f; }
+        }
+        acc[i & 1] = f2_add(acc[i & 1], f2_pack(e0, e1));
+      }
+    };
+    int v = slice.v0 + tid;
+    for (; v + DT_THREADS < slice.v1; v += 2 * DT_THREADS) {
+      const uint4 u0 = __ldg(xv + v), u1 = __ldg(xv + v + DT_THREADS);
+      sum(u0, v);
+      sum(u1, v + DT_THREADS);
     }
-    sR = block_reduce<DT_WARPS>(sR, OpSum(), s.wf);
-    sS = block_reduce<DT_WARPS>(sS, OpSum(), s.wf);
-    lR = aR + logf(sR);
-    const float lS = aS + logf(sS);
-    l = m == -INFINITY ? m : m + logf(expf(lR - m) + expf(lS - m));
-    const double pt = p.teacher_lse && t.live && count < V ? fmax(0.0, 1.0 - t.psum) : 0.0;
-    const double T2 = (double)p.temperature * (double)p.temperature;
-    double loss = 0.0;
+    if (v < slice.v1) sum(__ldg(xv + v), v);
+    for (int i = tid; i < slice.n_single(rank, blocks); i += DT_THREADS) {
+      const int j = slice.single(i, rank);
+      const float z = Z(to_float(x[j]));
+      if (flag(j)) sS += exp2_approx(z - mS);
+      else sR += exp2_approx(z - mR);
+    }
+    {
+      float a0, a1;
+      f2_unpack(f2_add(acc[0], acc[1]), a0, a1);
+      sR += a0 + a1;
+    }
+    // the teacher's side of the sums
+    double E = 0.0, F = 0.0;   // sum of e_k, and of e_k (t_k - z_k)
     for (int k = tid; k < K; k += DT_THREADS) {
-      const float pk = s.p[k];
-      if (!(pk == 0.f)) loss += (double)pk * ((double)p.values[row * K + k] / (double)p.temperature - t.L - (double)z_of(to_float(x[s.id[k]])) + (double)l);
+      double e = 0.0;
+      if (en.id[k] >= 0 && live) {
+        e = exp(en.t[k] - L);
+        if (!(e == 0.0)) F += e * (en.t[k] - (double)en.z[k] * DT_LN2);
+      }
+      en.e[k] = (float)e;
+      E += e;
     }
-    loss = block_reduce<DT_WARPS>(loss, OpSum(), s.wd);
-    if (!(pt == 0.0)) loss += pt * (log(pt) - (double)lR + (double)l);
-    W = (float)(t.psum + pt);
-    B = lR == -INFINITY ? 0.f : (float)((double)W * exp((double)lR - (double)l) - pt);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sR += __shfl_xor_sync(0xffffffffu, sR, o);
+      sS += __shfl_xor_sync(0xffffffffu, sS, o);
+      E += __shfl_xor_sync(0xffffffffu, E, o);
+      F += __shfl_xor_sync(0xffffffffu, F, o);
+    }
+    __syncthreads();
+    if (lane == 0) { s.wf[0][warp] = sR; s.wf[1][warp] = sS; s.wd[0][warp] = E; s.wd[1][warp] = F; }
+    __syncthreads();
+    if (blocks > 1) {
+      sR = sS = 0.f;
+      for (int w = 0; w < DT_WARPS; ++w) { sR += s.wf[0][w]; sS += s.wf[1][w]; }
+      if (tid < blocks) st_cluster_f32(mapa_u32(smem_u32(s.from[1] + rank), tid), sS);
+      sR = dt_exchange(sR, s.from[0], rank, blocks, OpSum());
+    }
     if (tid == 0) {
-      p.loss[row] = (float)(T2 * loss);
-      if (st) { st[ST_LR] = lR; st[ST_L] = l; st[ST_B] = B; st[ST_W] = W; }
+      if (blocks > 1) {
+        sS = 0.f;
+        for (int r = 0; r < blocks; ++r) sS += s.from[1][r];
+      } else {
+        sR = sS = 0.f;
+        for (int w = 0; w < DT_WARPS; ++w) { sR += s.wf[0][w]; sS += s.wf[1][w]; }
+      }
+      E = F = 0.0;
+      for (int w = 0; w < DT_WARPS; ++w) { E += s.wd[0][w]; F += s.wd[1][w]; }
+      const double lR = log2((double)sR) + (double)mR, lS = log2((double)sS) + (double)mS, top = fmax(lR, lS);   // log2(0) = -inf
+      const double l = top == -INFINITY ? top : top + log2(exp2(lR - top) + exp2(lS - top));
+      const double left = given && live && count < V ? fmax(0.0, 1.0 - E) : 0.0;   // p_tail
+      double loss = 0.0, W = 0.0;
+      if (live) {
+        W = given ? E + left : 1.0;
+        loss = given ? F + E * (l * DT_LN2 - L) : F / E + l * DT_LN2 - (L + log(E));
+        if (!(left == 0.0)) loss += left * (log(left) - (lR - l) * DT_LN2);
+      }
+      s.lR = lR == -INFINITY ? 0.f : (float)lR;
+      s.l = (float)l;
+      s.B = lR == -INFINITY ? 0.f : (float)(W * exp2(lR - l) - left);
+      s.W = (float)W;
+      s.pscale = given ? 1.f : (float)(1.0 / E);
+      if (rank == 0) {
+        p.loss[row] = (float)((double)p.temperature * (double)p.temperature * loss);
+        if (st) {
+          st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W;
+          *reinterpret_cast<double*>(st + ST_TEACHER) = given ? L : L + log(E);
+        }
+      }
     }
   } else {
-    lR = st[ST_LR]; l = st[ST_L]; B = st[ST_B]; W = st[ST_W];
+    for (int k = tid; k < K; k += DT_THREADS) en.e[k] = en.id[k] >= 0 && live ? (float)exp(en.t[k] - L) : 0.f;
+    if (tid == 0) { s.lR = st[ST_LR]; s.l = st[ST_L]; s.B = st[ST_B]; s.W = st[ST_W]; s.pscale = 1.f; }
   }
   if (!GRAD) return;
-  const float g = (p.weight ? p.weight[row * p.weight_stride] : 1.f) * p.temperature;
+  __syncthreads();
+
   T* dx = static_cast<T*>(p.dlogits) + row * p.dlogits_stride;
-  for (int j = tid; j < V; j += DT_THREADS) {
-    const float v = to_float(x[j]);
-    const float th = cap > 0.f ? dt_tanh(v, cap) : 0.f, z = (cap > 0.f ? cap * th : v) * invT;
-    if (!in_top(j)) dx[j] = from_float<T>(t.live ? g * B * expf(z - lR) * (1.f - th * th) : 0.f);
+  const bool wide = (reinterpret_cast<uintptr_t>(dx + slice.head) & 15u) == 0;   // the gradient's vectors lie like the logits'
+  const float g = live ? (p.weight ? p.weight[row * p.weight_stride] : 1.f) * p.temperature : 0.f, gB = g * s.B, lR = s.lR;
+  const float bend = CAP ? gB / (Z.a * Z.a) : 0.f;   // slope 1 - tanh^2 = 1 - (z / a)^2
+  const f32x2 gB2 = f2_dup(gB), bend2 = f2_dup(-bend), shift = f2_dup(-lR);
+  auto grad = [&](const uint4& u, int v) {
+    f32x2 d[N / 2];
+    if (live) {
+      Vec16<T> a;
+      a.set(u);
+      f32x2 z[N / 2];
+      Z.template of<T>(a, z);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        float e0, e1;
+        f2_unpack(f2_add(z[i], shift), e0, e1);
+        const f32x2 e = f2_pack(exp2_approx(e0), exp2_approx(e1));
+        d[i] = f2_mul(e, CAP ? f2_fma(f2_mul(z[i], z[i]), bend2, gB2) : gB2);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) d[i] = 0ull;
+    }
+    const uint4 out = Vec16<T>::round(d);
+    if (wide) {
+      __stcs(reinterpret_cast<uint4*>(dx + slice.head) + v, out);
+    } else {
+      const T* o = reinterpret_cast<const T*>(&out);
+#pragma unroll
+      for (int i = 0; i < N; ++i) dx[slice.element(v) + i] = o[i];
+    }
+  };
+  int v = slice.v0 + tid;
+  for (; v + DT_THREADS < slice.v1; v += 2 * DT_THREADS) {
+    const uint4 u0 = __ldcs(xv + v), u1 = __ldcs(xv + v + DT_THREADS);
+    grad(u0, v);
+    grad(u1, v + DT_THREADS);
   }
+  if (v < slice.v1) grad(__ldcs(xv + v), v);
+  for (int i = tid; i < slice.n_single(rank, blocks); i += DT_THREADS) {
+    const int j = slice.single(i, rank);
+    const float z = Z(to_float(x[j]));
+    dx[j] = from_float<T>(live ? exp2_approx(z - lR) * (CAP ? fmaf(-bend * z, z, gB) : gB) : 0.f);
+  }
+  __syncthreads();   // the named tokens got the tail's gradient, too: theirs follows
+  const float l = s.l, W = s.W, flat = CAP ? 1.f / (Z.a * Z.a) : 0.f;
   for (int k = tid; k < K; k += DT_THREADS) {
-    const int id = s.id[k];
-    if (id < 0) continue;
-    const float v = to_float(x[id]);
-    const float th = cap > 0.f ? dt_tanh(v, cap) : 0.f, z = (cap > 0.f ? cap * th : v) * invT;
-    float pk = 0.f;
-    for (int i = 0; i < K; ++i) pk += s.id[i] == id ? s.p[i] : 0.f;   // (every entry of a token named twice writes the same value)
-    dx[id] = from_float<T>(t.live ? g * (W * expf(z - l) - pk) * (1.f - th * th) : 0.f);
+    const int id = en.id[k];
+    if (id < 0 || !live) continue;
+    const int o = slice.place(id);
+    if (o < slice.first || o >= slice.end) continue;
+    float pk = en.e[k];
+    if (again) {   // a token named twice: all its entries write the same value
+      pk = 0.f;
+      for (int i = 0; i < K; ++i) pk += en.id[i] == id ? en.e[i] : 0.f;
+    }
+    const float z = en.z[k];
+    dx[id] = from_float<T>(g * (W * exp2_approx(z - l) - pk * s.pscale) * (CAP ? 1.f - flat * z * z : 1.f));
   }
 }
 
@@ -156,8 +333,9 @@ static int dt_validate(const xl_distill_params* p) {
   if (!p || !p->logits || !p->values || !p->ids) return XL_ERR_NULL_POINTER;
   const int rc = vocab_validate(p->rows, p->V, p->row_stride, p->cap, p->dtype);
   if (rc != XL_OK) return rc;
-  if (p->K <= 0 || !(p->temperature > 0.f) || p->temperature > 3.0e38f) return XL_ERR_BAD_SHAPE;
+  if (p->K <= 0 || !vocab_temperature(p->temperature)) return XL_ERR_BAD_SHAPE;
   if (p->K > TOPK_MAX) return XL_ERR_TOO_LARGE;
+  if (p->stats && (reinterpret_cast<uintptr_t>(p->stats) & 7u)) return XL_ERR_BAD_ALIGNMENT;
   if (p->dlogits && p->rows > 1 && p->dlogits_stride < p->V) return XL_ERR_BAD_STRIDE;
   if (p->dlogits) {
     const uintptr_t size = p->dtype == XL_F32 ? 4 : 2, n = (uintptr_t)p->V * size, last = (uintptr_t)(p->rows - 1) * size;
@@ -167,15 +345,42 @@ static int dt_validate(const xl_distill_params* p) {
   return XL_OK;
 }
 
+// Blocks of a row.  One fills the machine from 592 rows on (four blocks an SM); fewer rows are cut into up to eight slices
+// of at least 2048 tokens that exchange their sums through the cluster's shared memory.
+static int dt_blocks(int rows, int V) {
+  int blocks = 1;
+  while (blocks < 8 && rows * (blocks * 2) <= 4 * 148 && V >= 2048 * (blocks * 2)) blocks *= 2;
+  return blocks;
+}
+
+template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD> static int dt_go(const xl_distill_params* p, cudaStream_t st) {
+  const int blocks = dt_blocks(p->rows, p->V);
+  auto kern = distill_kernel<T, CAP, BOUNDED, LOSS, GRAD>;
+  const size_t smem = dt_smem(p->K, p->V, Vec16<T>::N, blocks);
+  if (smem > 40 * 1024) XL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p->rows * blocks);
+  cfg.blockDim = dim3(DT_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)blocks, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, *p, blocks));
+  return check_launch("xl_distill_topk");
+}
+
 template <typename T> static int dt_launch(const xl_distill_params* p, bool loss, cudaStream_t st) {
-  const size_t smem = (size_t)((p->V + 31) / 32) * 4;
-  auto go = [&](auto kern) -> int {
-    XL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, VOCAB_MAX / 8));
-    kern<<<p->rows, DT_THREADS, smem, st>>>(*p);
-    return check_launch("xl_distill_topk");
-  };
-  if (!loss) return go(distill_kernel<T, false, true>);
-  return p->dlogits ? go(distill_kernel<T, true, true>) : go(distill_kernel<T, true, false>);
+  const bool cap = p->cap > 0.f, bounded = cap && 1.45 * (double)p->cap <= DT_BOUND * (double)p->temperature;
+  if (!loss) return cap ? dt_go<T, true, true, false, true>(p, st) : dt_go<T, false, false, false, true>(p, st);
+  if (p->dlogits) {
+    if (bounded) return dt_go<T, true, true, true, true>(p, st);
+    return cap ? dt_go<T, true, false, true, true>(p, st) : dt_go<T, false, false, true, true>(p, st);
+  }
+  if (bounded) return dt_go<T, true, true, true, false>(p, st);
+  return cap ? dt_go<T, true, false, true, false>(p, st) : dt_go<T, false, false, true, false>(p, st);
 }
 
 }  // namespace xl

@@ -61,10 +61,156 @@ struct OpSum {
   template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
 
+// ---------------------------------------------------------------------------------------------
+// fp32 arithmetic of the capped logits, two elements to an instruction
+//
+// Packed fma/mul/add take two cycles of the fp32 pipe but one issue slot for two elements (measured: 65 packed against 125
+// plain instructions per cycle and SM), and a row's passes are as much bound by issue slots as by the pipe.
+// ---------------------------------------------------------------------------------------------
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 f2_pack(float a, float b) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ f32x2 f2_bits(uint32_t a, uint32_t b) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ f32x2 f2_dup(float a) { return f2_pack(a, a); }
+__device__ __forceinline__ void f2_unpack(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 f2_fma(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// tanh(z) = z P(z^2) for |z| <= 0.75, relative error within 3 * 2^-24 (least-squares weights driven to the minimax, degree 5);
+// a model's logits stay below three quarters of the cap.  Beyond it 1 - 2 / (1 + e^2|z|), whose quotient is below 0.37 there.
+constexpr float TANH_SMALL = 0.75f;
+__device__ __forceinline__ float tanh_large(float z) {
+  const float q = 1.f - __fdividef(2.f, 1.f + exp2_approx(fminf(fabsf(z), 20.f) * (2.f * LOG2E)));
+  return z != z ? z : copysignf(q, z);
+}
+
+// A vector of 16 bytes of logits as packed fp32 pairs.
+template <typename T> struct Vec16;
+template <> struct Vec16<__nv_bfloat16> {
+  static constexpr int N = 8;
+  f32x2 p[4];
+  uint4 raw;
+  __device__ __forceinline__ void set(const uint4& u) {
+    raw = u;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = f2_bits(w[i] << 16, w[i] & 0xffff0000u);
+  }
+  __device__ __forceinline__ float largest() const {   // of the magnitudes; NaN does not count
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+    return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
+  }
+  static __device__ __forceinline__ uint4 round(const f32x2 (&v)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      f2_unpack(v[i], a, b);
+      w[i] = pack_bf16x2(a, b);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <> struct Vec16<float> {
+  static constexpr int N = 4;
+  f32x2 p[2];
+  __device__ __forceinline__ void set(const uint4& u) { p[0] = f2_bits(u.x, u.y); p[1] = f2_bits(u.z, u.w); }
+  __device__ __forceinline__ float largest() const {
+    float a, b, c, d;
+    f2_unpack(p[0], a, b);
+    f2_unpack(p[1], c, d);
+    return fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d)));
+  }
+  static __device__ __forceinline__ uint4 round(const f32x2 (&v)[2]) {
+    uint4 u;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(u.x), "=r"(u.y) : "l"(v[0]));
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(u.z), "=r"(u.w) : "l"(v[1]));
+    return u;
+  }
+};
+
+// z = a * tanh(x / cap) with a = cap log2(e) / T, or x * log2(e) / T without a cap: exponents of two.
+template <bool CAP> struct CappedZ {
+  float a, icap, c0, c1, c2, c3, c4, c5;
+  __device__ __forceinline__ CappedZ(float cap, float temperature) {
+    const double scale = 1.4426950408889634 / (double)temperature;
+    a = (float)(CAP ? scale * (double)cap : scale);
+    icap = CAP ? 1.f / cap : 0.f;
+    c0 = a; c1 = a * -0.33332958817481995f; c2 = a * 0.1332540661096573f; c3 = a * -0.05334443226456642f; c4 = a * 0.01958290860056877f;
+    c5 = a * -0.004716257099062204f;
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    if (!CAP) return x * a;
+    const float z = x * icap, s = z * z;
+    if (fabsf(z) > TANH_SMALL) return a * tanh_large(z);
+    return z * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, c5, c4), c3), c2), c1), c0);
+  }
+  template <typename T> __device__ __forceinline__ void of(const Vec16<T>& v, f32x2 (&out)[Vec16<T>::N / 2]) const {
+    if (!CAP) {
+#pragma unroll
+      for (int i = 0; i < Vec16<T>::N / 2; ++i) out[i] = f2_mul(v.p[i], f2_dup(a));
+      return;
+    }
+    if (v.largest() * icap <= TANH_SMALL) {
+#pragma unroll
+      for (int i = 0; i < Vec16<T>::N / 2; ++i) {
+        const f32x2 z = f2_mul(v.p[i], f2_dup(icap)), s = f2_mul(z, z);
+        f32x2 q = f2_fma(s, f2_dup(c5), f2_dup(c4));
+        q = f2_fma(s, q, f2_dup(c3));
+        q = f2_fma(s, q, f2_dup(c2));
+        q = f2_fma(s, q, f2_dup(c1));
+        out[i] = f2_mul(z, f2_fma(s, q, f2_dup(c0)));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::N / 2; ++i) {
+      float x0, x1;
+      f2_unpack(v.p[i], x0, x1);
+      out[i] = f2_pack((*this)(x0), (*this)(x1));
+    }
+  }
+};
+
+// How a row that may start anywhere lies in 16-byte vectors, and which of them are this block's: `head` elements in front of
+// the first boundary (block 0 of the row), vectors [v0, v1), and the rest behind the last vector (the last block).
+// place(j) numbers the elements so that vector v holds N (v + 1) .. N (v + 1) + N - 1.
+template <typename T> struct RowSlice {
+  static constexpr int N = Vec16<T>::N;
+  int head, vectors, v0, v1, first, end;   // places [first, end) are this block's
+  int V;
+  __device__ __forceinline__ RowSlice(const T* x, int V_, int rank, int blocks) : V(V_) {
+    const int mis = (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % N);
+    head = min(V, mis ? N - mis : 0);
+    vectors = (V - head) / N;
+    const int per = (vectors + blocks - 1) / blocks;
+    v0 = min(vectors, rank * per);
+    v1 = min(vectors, v0 + per);
+    first = rank == 0 ? 0 : N * (v0 + 1);
+    end = rank == blocks - 1 ? place(V) : N * (v1 + 1);
+  }
+  __device__ __forceinline__ int place(int j) const { return j - head + N; }
+  __device__ __forceinline__ int element(int v) const { return head + v * N; }
+  // places of the block's single elements: n_single of them, the i-th is element single(i)
+  __device__ __forceinline__ int n_single(int rank, int blocks) const {
+    return (rank == 0 ? head : 0) + (rank == blocks - 1 ? V - head - vectors * N : 0);
+  }
+  __device__ __forceinline__ int single(int i, int rank) const {
+    const int h = rank == 0 ? head : 0;
+    return i < h ? i : head + vectors * N + i - h;
+  }
+};
+
+// temperatures of the entries that compute in fp32
+static inline bool vocab_temperature(float t) { return t >= 1e-4f && t <= 1e6f; }
 // what row-wise entries over logits check in common
 static inline int vocab_validate(int rows, int V, int64_t row_stride, float cap, int dtype) {
   if (dtype != XL_F32 && dtype != XL_BF16) return XL_ERR_BAD_DTYPE;
-  if (rows <= 0 || V <= 0 || !(cap >= 0.f) || cap > 3.0e38f) return XL_ERR_BAD_SHAPE;
+  if (rows <= 0 || V <= 0 || !(cap == 0.f || (cap >= 1e-6f && cap <= 1e6f))) return XL_ERR_BAD_SHAPE;
   if (rows > 1 && row_stride < V) return XL_ERR_BAD_STRIDE;
   if (V > VOCAB_MAX) return XL_ERR_TOO_LARGE;
   return XL_OK;

@@ -123,7 +123,7 @@ extern "C" int xl_softcap_topk(const xl_topk_params* p, void* cuda_stream) {
   if (!p || !p->logits || !p->values || !p->ids) return XL_ERR_NULL_POINTER;
   int rc = vocab_validate(p->rows, p->V, p->row_stride, p->cap, p->dtype);
   if (rc != XL_OK) return rc;
-  if (p->k <= 0 || p->k > p->V || !(p->temperature > 0.f) || p->temperature > 3.0e38f) return XL_ERR_BAD_SHAPE;
+  if (p->k <= 0 || p->k > p->V || !vocab_temperature(p->temperature)) return XL_ERR_BAD_SHAPE;
   if (p->k > TOPK_MAX) return XL_ERR_TOO_LARGE;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   if (p->dtype == XL_F32) topk_kernel<float><<<p->rows, TK_THREADS, 0, st>>>(*p);
