@@ -467,7 +467,7 @@ typedef struct xl_sample_params {
   int32_t dtype;
 } xl_sample_params;
 
-/* Requires V <= 2^19.  Needs no scratch memory; calls may overlap. */
+/* Requires V <= 2^18.  Needs no scratch memory; calls may overlap. */
 int xl_softcap_sample(const xl_sample_params* p, void* cuda_stream);
 
 /* ------------------------------------------------------------------------------------------------
@@ -480,7 +480,7 @@ typedef struct xl_topk_params {
   float* values;            /* out (rows, k): y, not divided by the temperature */
   int32_t* ids;             /* out (rows, k) */
   float* lse;               /* out (rows) or NULL */
-  int32_t rows, V, k;       /* 1 <= k <= min(V, 1024), V <= 2^19 */
+  int32_t rows, V, k;       /* 1 <= k <= min(V, 1024), V <= 2^18 */
   int64_t row_stride;
   float cap;                /* 1e-6 .. 1e6; 0: none */
   float temperature;        /* 1e-4 .. 1e6 */
@@ -511,7 +511,7 @@ typedef struct xl_distill_params {
   float* stats;             /* (rows, 8) fp32, 8-byte aligned, what the backward entry needs: out of xl_distill_topk (or NULL), in for
                                xl_distill_topk_backward */
   int32_t* status;          /* device word or NULL */
-  int32_t rows, V, K;       /* 1 <= K <= 1024, V <= 2^19 */
+  int32_t rows, V, K;       /* 1 <= K <= 1024, V <= 2^18 */
   int32_t ids64;
   int64_t row_stride, dlogits_stride, weight_stride;
   float cap;                /* 1e-6 .. 1e6; 0: none */

@@ -474,4 +474,4 @@ def test_vocab_refusals():
     with pytest.raises(XlError, match="capacity"):
         xlstm_b200.distill_topk(wide, torch.zeros(1, 1025).cuda(), torch.zeros(1, 1025, dtype=torch.int32).cuda())
     with pytest.raises(XlError, match="capacity"):
-        xlstm_b200.softcap_sample(torch.zeros(1, 2 ** 19 + 1).cuda(), None, u[:1])
+        xlstm_b200.softcap_sample(torch.zeros(1, 2 ** 18 + 1).cuda(), None, u[:1])

@@ -37,7 +37,7 @@ def test_entries_check_before_they_launch():
     assert l.xl_softcap_sample(ref(s), None) == -2      # negative cap
     s.cap, s.row_stride = 0.0, 7
     assert l.xl_softcap_sample(ref(s), None) == -3      # rows overlap
-    s.V = s.row_stride = 2 ** 19 + 1
+    s.V = s.row_stride = 2 ** 18 + 1
     assert l.xl_softcap_sample(ref(s), None) == -8
     t = _lib.TopkParams()
     assert l.xl_softcap_topk(ref(t), None) == -1

@@ -12,18 +12,19 @@
 
 namespace xl {
 
-constexpr int DT_THREADS = 256, DT_WARPS = DT_THREADS / 32;
+constexpr int DT_THREADS = 256, DT_WARPS = DT_THREADS / 32, DT_BLOCKS = 8;
 constexpr double DT_LN2 = 0.69314718055994530942;
 // what a row leaves for its gradient; the last two places hold a double
-enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_LIVE = 4, ST_TEACHER = 6 };
+enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_SMALL = 4, ST_TEACHER = 6 };
 
 struct DtShared {
-  double wd[2][DT_WARPS];
-  float wf[2][DT_WARPS], from[3][8];   // from: of the row's blocks; a place is written once a launch
+  double wd[3][DT_WARPS];
+  float wf[2][DT_WARPS], from[4][DT_BLOCKS];   // from: of the row's blocks; a place is written once a launch
   int wi[2][DT_WARPS];
   float lR, l, B, W, pscale;
 };
-// behind it: K entries -- t / T, id (-1: unused), z of the student there, e^(t / T - shift) -- and a bit per token of the slice
+// Dynamic shared memory: K entries -- t / T, id (-1: unused), z of the student there, e^(t / T - shift) -- and a bit per token of
+// the slice.
 struct DtEntries {
   double* t;
   int* id;
@@ -38,109 +39,174 @@ struct DtEntries {
   }
 };
 static size_t dt_smem(int K, int V, int N, int blocks) {
-  const size_t vectors = (size_t)V / N, places = ((vectors + blocks - 1) / blocks + 3) * N;
-  return (size_t)K * 20 + (places + 31) / 32 * 4 + 4;
+  const size_t vectors = (size_t)V / N, per = (vectors + blocks - 1) / blocks;
+  return (size_t)K * 20 + ((per + 3) * N + 31) / 32 * 4 + 4;
 }
 
 // one value of every block of the row's cluster, in rank order, combined by `f`
 template <typename F> __device__ __forceinline__ float dt_exchange(float v, float* from, int rank, int blocks, F f) {
   if (threadIdx.x < blocks) st_cluster_f32(mapa_u32(smem_u32(from + rank), threadIdx.x), v);
+  __syncwarp();
   cluster_sync_all();
   v = from[0];
   for (int r = 1; r < blocks; ++r) v = f(v, from[r]);
   return v;
 }
 
-// Bound: with a cap |z| <= a, so that sums of 2^z need no maximum in front: 2^a * 2^19 and 2^-a stay normal numbers.
+// Bound: with a cap |z| <= a, so that sums of 2^z need no maximum in front: 2^a * 2^18 and 2^-a stay normal numbers.
 constexpr float DT_BOUND = 100.f;
 
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+// f(vector, its number) for v, v + STEP, .. below end, four loads under way at a time
+template <int STEP, typename F> __device__ __forceinline__ void dt_vectors(const uint4* xv, int v, int end, F f) {
+#pragma unroll 1
+  for (; v + 3 * STEP < end; v += 4 * STEP) {
+    uint4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __ldg(xv + v + i * STEP);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f(u[i], v + i * STEP);
+  }
+#pragma unroll 1
+  for (; v < end; v += STEP) f(__ldg(xv + v), v);
+}
+
+__device__ __forceinline__ double dt_nanmax(double a, double b) { return a != a || b != b ? a + b : fmax(a, b); }   // (NaN survives)
+
 template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(DT_THREADS) distill_kernel(const xl_distill_params p, const int blocks) {
+__global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill_params p, const CappedZ<CAP> Z, const double invT, const int blocks) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ DtShared s;
-  constexpr int N = Vec16<T>::N;
+  constexpr int N = Vec16<T>::N, THREADS = DT_THREADS, WARPS = DT_WARPS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, K = p.K;
   const int rank = blocks > 1 ? (int)cluster_ctarank() : 0;
   const long long row = blockIdx.x / blocks;
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
   const RowSlice<T> slice(x, V, rank, blocks);
   const uint4* xv = reinterpret_cast<const uint4*>(x + slice.head);
-  const CappedZ<CAP> Z(p.cap, p.temperature);
+  const int singles = slice.n_single(rank, blocks);
+  // (shared memory of another block may be written once that block runs: the other half of this barrier is in front of the first exchange)
+  if (LOSS && blocks > 1) cluster_arrive();
   const DtEntries en(dynamic, K);
   const bool given = p.teacher_lse != nullptr;
   float* st = p.stats ? p.stats + row * 8 : nullptr;
-  const unsigned char* bytes = reinterpret_cast<const unsigned char*>(en.bits);
+  const unsigned char* bytes = reinterpret_cast<const unsigned char*>(en.bits) + (N == 8 ? 1 - slice.first / 8 : 0);
   auto flags = [&](int v) -> unsigned int {   // bits of the vector's elements
+    if (N == 8) return bytes[v];
     const int o = N * (v + 1) - slice.first;
-    return N == 8 ? bytes[o >> 3] : (unsigned int)(bytes[o >> 3] >> (o & 4)) & 15u;
+    return (unsigned int)(bytes[o >> 3] >> (o & 4)) & 15u;
   };
   auto flag = [&](int j) -> bool {
     const int o = slice.place(j) - slice.first;
     return (en.bits[o >> 5] >> (o & 31)) & 1u;
   };
 
-  // (shared memory of another block may be written once that block runs: the other half of this barrier is in front of the first exchange)
-  if (LOSS && blocks > 1) cluster_arrive();
   // the teacher's entries, the student's logits there, and the bits of the tokens named
-  for (int w = tid; w < (slice.end - slice.first + 31) / 32; w += DT_THREADS) en.bits[w] = 0u;
-  __syncthreads();
-  const double invT = 1.0 / (double)p.temperature;
+  if (LOSS) {
+    for (int w = tid; w < (slice.end - slice.first + 31) / 32; w += THREADS) en.bits[w] = 0u;
+    __syncthreads();
+  }
+  const int with = min(WARPS, (K + 31) / 32);   // warps that have entries
   double m = -INFINITY;   // of t / T
   float mS = -INFINITY;
   int any = 0, twice = 0, count = 0;
-  for (int k = tid; k < K; k += DT_THREADS) {
-    const long long at = row * K + k, id = p.ids64 ? static_cast<const int64_t*>(p.ids)[at] : (long long)static_cast<const int32_t*>(p.ids)[at];
-    const bool used = id >= 0 && id < V;
-    if (id >= V && p.status) atomicExch(p.status, 4);
-    en.id[k] = used ? (int)id : -1;
-    en.z[k] = 0.f;
-    if (!used) continue;
-    const double t = (double)p.values[at] * invT;
-    en.t[k] = t;
-    any = 1;
-    m = t != t || m != m ? t + m : fmax(m, t);   // (NaN survives)
-    en.z[k] = Z(to_float(x[id]));
-    mS = fmaxf(mS, en.z[k]);
-    const int o = slice.place((int)id) - slice.first;
-    if (o >= 0 && o < slice.end - slice.first) {
-      const int old = (atomicOr(&en.bits[o >> 5], 1u << (o & 31)) >> (o & 31)) & 1u;
-      twice |= old;
-      count += 1 - old;
+  if (warp < with) {
+    for (int k = tid; k < K; k += THREADS) {
+      const long long at = row * K + k, id = p.ids64 ? static_cast<const int64_t*>(p.ids)[at] : (long long)static_cast<const int32_t*>(p.ids)[at];
+      const double t = (double)p.values[at] * invT;
+      const bool used = id >= 0 && id < V;
+      if (id >= V && p.status) atomicExch(p.status, 4);
+      en.id[k] = used ? (int)id : -1;
+      en.z[k] = 0.f;
+      if (!used) continue;
+      en.t[k] = t;
+      any = 1;
+      m = dt_nanmax(m, t);
+      en.z[k] = Z(to_float(x[id]));
+      mS = fmaxf(mS, en.z[k]);
+      const int o = slice.place((int)id) - slice.first;
+      if (LOSS && o >= 0 && o < slice.end - slice.first) {
+        const int old = (atomicOr(&en.bits[o >> 5], 1u << (o & 31)) >> (o & 31)) & 1u;
+        twice |= old;
+        count += 1 - old;
+      }
+    }
+    if (LOSS) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        m = dt_nanmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!BOUNDED) mS = fmaxf(mS, __shfl_xor_sync(0xffffffffu, mS, o));
+      }
+      if (K >= V) count = __reduce_add_sync(0xffffffffu, count);
+    }
+    any = (__any_sync(0xffffffffu, any) ? 1 : 0) | (__any_sync(0xffffffffu, twice) ? 2 : 0);
+    if (lane == 0) { s.wd[2][warp] = m; s.wf[0][warp] = mS; s.wi[0][warp] = any; s.wi[1][warp] = count; }
+  }
+  __syncthreads();   // (the bits are there, too)
+  any = 0;
+  count = 0;
+  for (int w = 0; w < with; ++w) {
+    if (LOSS) {
+      m = dt_nanmax(m, s.wd[2][w]);
+      if (!BOUNDED) mS = fmaxf(mS, s.wf[0][w]);
+      count += s.wi[1][w];
+    }
+    any |= s.wi[0][w];
+  }
+  const bool everything = K >= V && count == V;   // no token is left for the tail
+  bool again = any & 2, live = any & 1;
+  double L = 0.0;   // shift of the teacher's exponents; with its own sum, or in the backward pass, the right one from the start
+  if (LOSS) {
+    live = live && (given || m != -INFINITY);
+    if (live) L = given ? (double)p.teacher_lse[row] : m;
+  } else {
+    live = live && st[ST_W] != 0.f;
+    again = true;   // (not known here)
+    L = *reinterpret_cast<const double*>(st + ST_TEACHER);
+  }
+  mS = BOUNDED || mS == -INFINITY ? 0.f : mS;
+  float sS = 0.f;   // of the slice's tokens named
+  if (warp < with) {
+    double E = 0.0, F = 0.0;   // sum of e_k, and of e_k (t_k - z_k)
+    for (int k = tid; k < K; k += THREADS) {
+      double e = 0.0;
+      if (en.id[k] >= 0 && live) {
+        e = exp(en.t[k] - L);
+        if (LOSS && !(e == 0.0)) F += e * (en.t[k] - (double)en.z[k] * DT_LN2);
+      }
+      en.e[k] = (float)e;
+      E += e;
+      if (LOSS && en.id[k] >= 0) {
+        const int o = slice.place(en.id[k]);
+        bool first = o >= slice.first && o < slice.end;
+        if (again)   // a token named twice is summed once
+          for (int i = 0; i < k; ++i) first = first && en.id[i] != en.id[k];
+        if (first) sS += exp2_approx(en.z[k] - mS);
+      }
+    }
+    if (LOSS) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        E += __shfl_xor_sync(0xffffffffu, E, o);
+        F += __shfl_xor_sync(0xffffffffu, F, o);
+        sS += __shfl_xor_sync(0xffffffffu, sS, o);
+      }
+      if (lane == 0) { s.wd[0][warp] = E; s.wd[1][warp] = F; s.wf[1][warp] = sS; }
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double om = __shfl_xor_sync(0xffffffffu, m, o);
-    m = om != om || m != m ? om + m : fmax(m, om);
-    mS = fmaxf(mS, __shfl_xor_sync(0xffffffffu, mS, o));
-    count += __shfl_xor_sync(0xffffffffu, count, o);
-  }
-  any = __any_sync(0xffffffffu, any) | (__any_sync(0xffffffffu, twice) << 1);
-  if (lane == 0) { s.wd[0][warp] = m; s.wf[0][warp] = mS; s.wi[0][warp] = any; s.wi[1][warp] = count; }
-  __syncthreads();   // (the bits are there, too)
-  any = 0; count = 0;
-#pragma unroll
-  for (int w = 0; w < DT_WARPS; ++w) {
-    m = w == 0 ? s.wd[0][0] : s.wd[0][w] != s.wd[0][w] || m != m ? s.wd[0][w] + m : fmax(m, s.wd[0][w]);
-    mS = w == 0 ? s.wf[0][0] : fmaxf(mS, s.wf[0][w]);
-    any |= s.wi[0][w];
-    count += s.wi[1][w];
-  }
-  const bool again = any & 2, live = (any & 1) && (given || m != -INFINITY);
-  double L = 0.0;   // shift of the teacher's exponents; with its own sum, or in the backward pass, the right one from the start
-  if (live) {
-    if (!LOSS) L = *reinterpret_cast<const double*>(st + ST_TEACHER);
-    else L = given ? (double)p.teacher_lse[row] : m;
-  }
 
+  bool small = true;   // (this thread's) logits stay below three quarters of the cap
   if (LOSS) {
+    __syncwarp();
     if (blocks > 1) cluster_wait();
     float mR = 0.f;
     if (!BOUNDED) {
       float xm = -INFINITY;
-      for (int v = slice.v0 + tid; v < slice.v1; v += DT_THREADS) {
+      dt_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) {
         Vec16<T> a;
-        a.set(__ldg(xv + v));
+        a.set(u);
         const unsigned int f = flags(v);
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
@@ -149,121 +215,116 @@ __global__ void __launch_bounds__(DT_THREADS) distill_kernel(const xl_distill_pa
           if (!(f >> (2 * i) & 1u)) xm = fmaxf(xm, x0);
           if (!(f >> (2 * i + 1) & 1u)) xm = fmaxf(xm, x1);
         }
-      }
-      for (int i = tid; i < slice.n_single(rank, blocks); i += DT_THREADS) {
+      });
+      for (int i = tid; i < singles; i += THREADS) {
         const int j = slice.single(i, rank);
         if (!flag(j)) xm = fmaxf(xm, to_float(x[j]));
       }
-      xm = block_reduce<DT_WARPS>(xm, OpMax(), s.wf[1]);
+      xm = block_reduce<WARPS>(xm, OpMax(), s.wf[0]);
       if (blocks > 1) xm = dt_exchange(xm, s.from[2], rank, blocks, OpMax());
       mR = xm == -INFINITY ? 0.f : Z(xm);
-      mS = mS == -INFINITY ? 0.f : mS;
-    } else {
-      mS = 0.f;
     }
-    // both sums over the slice
-    float sR = 0.f, sS = 0.f;
+    // both sums over the slice.  The first try takes every magnitude for a small one and looks at the largest behind it;
+    // a thread that met a large one sums its vectors again.
+    float sR = 0.f;
     f32x2 acc[2] = {0ull, 0ull};
     const f32x2 shift = f2_dup(-mR);
-    auto sum = [&](const uint4& u, int v) {
+    typename Vec16<T>::Mag mag = Vec16<T>::no_mag();
+    auto sum = [&](auto is_small, const uint4& u, int v) {
       Vec16<T> a;
       a.set(u);
+      if (CAP && decltype(is_small)::value) mag = a.track(mag);
       f32x2 z[N / 2];
-      Z.template of<T>(a, z);
+      Z.template of<decltype(is_small)::value, T>(a, z);
       const unsigned int f = flags(v);
+      if (f != 0u) {   // (K of V tokens; their part is summed with the entries)
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float z0, z1;
+          f2_unpack(z[i], z0, z1);
+          z[i] = f2_pack(f >> (2 * i) & 1u ? -INFINITY : z0, f >> (2 * i + 1) & 1u ? -INFINITY : z1);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) {
         float z0, z1;
         f2_unpack(BOUNDED ? z[i] : f2_add(z[i], shift), z0, z1);
-        float e0 = exp2_approx(z0), e1 = exp2_approx(z1);
-        if (f) {   // (rare: K of V tokens)
-          f2_unpack(z[i], z0, z1);
-          if (f >> (2 * i) & 1u) { sS += exp2_approx(z0 - mS); e0 = 0.f; }
-          if (f >> (2 * i + 1) & 1u) { sS += exp2_approx(z1 - mS); e1 = 0.f; }
-        }
-        acc[i & 1] = f2_add(acc[i & 1], f2_pack(e0, e1));
+        acc[i & 1] = f2_add(acc[i & 1], f2_pack(exp2_approx(z0), exp2_approx(z1)));
       }
     };
-    int v = slice.v0 + tid;
-    for (; v + DT_THREADS < slice.v1; v += 2 * DT_THREADS) {
-      const uint4 u0 = __ldg(xv + v), u1 = __ldg(xv + v + DT_THREADS);
-      sum(u0, v);
-      sum(u1, v + DT_THREADS);
+    dt_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) { sum(Yes(), u, v); });
+    small = Z.small(Vec16<T>::largest(mag));
+    if (!small) {
+      sR = 0.f;
+      acc[0] = acc[1] = 0ull;
+#pragma unroll 1
+      for (int v = slice.v0 + tid; v < slice.v1; v += THREADS) sum(No(), __ldg(xv + v), v);
     }
-    if (v < slice.v1) sum(__ldg(xv + v), v);
-    for (int i = tid; i < slice.n_single(rank, blocks); i += DT_THREADS) {
+    for (int i = tid; i < singles; i += THREADS) {
       const int j = slice.single(i, rank);
       const float z = Z(to_float(x[j]));
-      if (flag(j)) sS += exp2_approx(z - mS);
-      else sR += exp2_approx(z - mR);
+      if (!flag(j)) sR += exp2_approx(z - mR);
     }
     {
       float a0, a1;
       f2_unpack(f2_add(acc[0], acc[1]), a0, a1);
       sR += a0 + a1;
     }
-    // the teacher's side of the sums
-    double E = 0.0, F = 0.0;   // sum of e_k, and of e_k (t_k - z_k)
-    for (int k = tid; k < K; k += DT_THREADS) {
-      double e = 0.0;
-      if (en.id[k] >= 0 && live) {
-        e = exp(en.t[k] - L);
-        if (!(e == 0.0)) F += e * (en.t[k] - (double)en.z[k] * DT_LN2);
-      }
-      en.e[k] = (float)e;
-      E += e;
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      sR += __shfl_xor_sync(0xffffffffu, sR, o);
-      sS += __shfl_xor_sync(0xffffffffu, sS, o);
-      E += __shfl_xor_sync(0xffffffffu, E, o);
-      F += __shfl_xor_sync(0xffffffffu, F, o);
-    }
+    for (int o = 16; o > 0; o >>= 1) sR += __shfl_xor_sync(0xffffffffu, sR, o);
+    int all_small = __syncthreads_and(small);   // (and the maximum in s.wf[0] has been read)
+    if (lane == 0) s.wf[0][warp] = sR;
     __syncthreads();
-    if (lane == 0) { s.wf[0][warp] = sR; s.wf[1][warp] = sS; s.wd[0][warp] = E; s.wd[1][warp] = F; }
-    __syncthreads();
-    if (blocks > 1) {
+    if (warp == 0) {
       sR = sS = 0.f;
-      for (int w = 0; w < DT_WARPS; ++w) { sR += s.wf[0][w]; sS += s.wf[1][w]; }
-      if (tid < blocks) st_cluster_f32(mapa_u32(smem_u32(s.from[1] + rank), tid), sS);
+      for (int w = 0; w < WARPS; ++w) sR += s.wf[0][w];
+      for (int w = 0; w < with; ++w) sS += s.wf[1][w];
+    }
+    if (blocks > 1) {
+      if (tid < blocks) {
+        st_cluster_f32(mapa_u32(smem_u32(s.from[1] + rank), tid), sS);
+        st_cluster_f32(mapa_u32(smem_u32(s.from[3] + rank), tid), (float)all_small);
+      }
       sR = dt_exchange(sR, s.from[0], rank, blocks, OpSum());
     }
-    if (tid == 0) {
+    if (warp == 0) {
       if (blocks > 1) {
         sS = 0.f;
-        for (int r = 0; r < blocks; ++r) sS += s.from[1][r];
-      } else {
-        sR = sS = 0.f;
-        for (int w = 0; w < DT_WARPS; ++w) { sR += s.wf[0][w]; sS += s.wf[1][w]; }
+        for (int r = 0; r < blocks; ++r) { sS += s.from[1][r]; all_small = all_small && s.from[3][r] > 0.f; }
       }
-      E = F = 0.0;
-      for (int w = 0; w < DT_WARPS; ++w) { E += s.wd[0][w]; F += s.wd[1][w]; }
-      const double lR = log2((double)sR) + (double)mR, lS = log2((double)sS) + (double)mS, top = fmax(lR, lS);   // log2(0) = -inf
-      const double l = top == -INFINITY ? top : top + log2(exp2(lR - top) + exp2(lS - top));
-      const double left = given && live && count < V ? fmax(0.0, 1.0 - E) : 0.0;   // p_tail
-      double loss = 0.0, W = 0.0;
-      if (live) {
-        W = given ? E + left : 1.0;
-        loss = given ? F + E * (l * DT_LN2 - L) : F / E + l * DT_LN2 - (L + log(E));
-        if (!(left == 0.0)) loss += left * (log(left) - (lR - l) * DT_LN2);
-      }
-      s.lR = lR == -INFINITY ? 0.f : (float)lR;
-      s.l = (float)l;
-      s.B = lR == -INFINITY ? 0.f : (float)(W * exp2(lR - l) - left);
-      s.W = (float)W;
-      s.pscale = given ? 1.f : (float)(1.0 / E);
-      if (rank == 0) {
-        p.loss[row] = (float)((double)p.temperature * (double)p.temperature * loss);
-        if (st) {
-          st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W;
-          *reinterpret_cast<double*>(st + ST_TEACHER) = given ? L : L + log(E);
+      double E = 0.0, F = 0.0;
+      for (int w = 0; w < with; ++w) { E += s.wd[0][w]; F += s.wd[1][w]; }
+      const double left = given && live && !everything ? fmax(0.0, 1.0 - E) : 0.0;   // p_tail
+      // sums in one scale, and the four logarithms in four lanes
+      const float top = BOUNDED ? 0.f : sR > 0.f ? (sS > 0.f ? fmaxf(mR, mS) : mR) : mS;
+      const double tR = BOUNDED || sR == 0.f ? sR : sR * exp2_approx(mR - top), tS = BOUNDED || sS == 0.f ? sS : sS * exp2_approx(mS - top);
+      const double lg = log2(lane == 0 ? (double)sR : lane == 1 ? tR + tS : lane == 2 ? E : left);
+      const double lR = __shfl_sync(0xffffffffu, lg, 0) + (double)mR, l = __shfl_sync(0xffffffffu, lg, 1) + (double)top;   // log2(0) = -inf
+      const double lE = __shfl_sync(0xffffffffu, lg, 2), lleft = __shfl_sync(0xffffffffu, lg, 3);
+      if (lane == 0) {
+        double loss = 0.0, W = 0.0;
+        if (live) {
+          W = given ? E + left : 1.0;
+          loss = given ? F + E * (l * DT_LN2 - L) : F / E + (l - lE) * DT_LN2 - L;
+          if (!(left == 0.0)) loss += left * (lleft - lR + l) * DT_LN2;
+        }
+        s.lR = sR == 0.f ? 0.f : (float)lR;
+        s.l = (float)l;
+        s.B = sR == 0.f ? 0.f : (float)(W * (tR / (tR + tS)) - left);
+        s.W = (float)W;
+        s.pscale = given ? 1.f : (float)(1.0 / E);
+        if (rank == 0) {
+          p.loss[row] = (float)((double)p.temperature * (double)p.temperature * loss);
+          if (st) {
+            st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W; st[ST_SMALL] = all_small ? 1.f : 0.f;
+            *reinterpret_cast<double*>(st + ST_TEACHER) = given ? L : L + lE * DT_LN2;
+          }
         }
       }
     }
   } else {
-    for (int k = tid; k < K; k += DT_THREADS) en.e[k] = en.id[k] >= 0 && live ? (float)exp(en.t[k] - L) : 0.f;
     if (tid == 0) { s.lR = st[ST_LR]; s.l = st[ST_L]; s.B = st[ST_B]; s.W = st[ST_W]; s.pscale = 1.f; }
+    small = st[ST_SMALL] > 0.f;
   }
   if (!GRAD) return;
   __syncthreads();
@@ -271,27 +332,9 @@ __global__ void __launch_bounds__(DT_THREADS) distill_kernel(const xl_distill_pa
   T* dx = static_cast<T*>(p.dlogits) + row * p.dlogits_stride;
   const bool wide = (reinterpret_cast<uintptr_t>(dx + slice.head) & 15u) == 0;   // the gradient's vectors lie like the logits'
   const float g = live ? (p.weight ? p.weight[row * p.weight_stride] : 1.f) * p.temperature : 0.f, gB = g * s.B, lR = s.lR;
-  const float bend = CAP ? gB / (Z.a * Z.a) : 0.f;   // slope 1 - tanh^2 = 1 - (z / a)^2
+  const float bend = CAP ? gB * Z.flat : 0.f;   // slope 1 - tanh^2 = 1 - (z / a)^2
   const f32x2 gB2 = f2_dup(gB), bend2 = f2_dup(-bend), shift = f2_dup(-lR);
-  auto grad = [&](const uint4& u, int v) {
-    f32x2 d[N / 2];
-    if (live) {
-      Vec16<T> a;
-      a.set(u);
-      f32x2 z[N / 2];
-      Z.template of<T>(a, z);
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        float e0, e1;
-        f2_unpack(f2_add(z[i], shift), e0, e1);
-        const f32x2 e = f2_pack(exp2_approx(e0), exp2_approx(e1));
-        d[i] = f2_mul(e, CAP ? f2_fma(f2_mul(z[i], z[i]), bend2, gB2) : gB2);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) d[i] = 0ull;
-    }
-    const uint4 out = Vec16<T>::round(d);
+  auto store = [&](const uint4& out, int v) {
     if (wide) {
       __stcs(reinterpret_cast<uint4*>(dx + slice.head) + v, out);
     } else {
@@ -300,21 +343,45 @@ __global__ void __launch_bounds__(DT_THREADS) distill_kernel(const xl_distill_pa
       for (int i = 0; i < N; ++i) dx[slice.element(v) + i] = o[i];
     }
   };
-  int v = slice.v0 + tid;
-  for (; v + DT_THREADS < slice.v1; v += 2 * DT_THREADS) {
-    const uint4 u0 = __ldcs(xv + v), u1 = __ldcs(xv + v + DT_THREADS);
-    grad(u0, v);
-    grad(u1, v + DT_THREADS);
+  auto grad = [&](const f32x2 (&z)[N / 2], int v) {
+    f32x2 d[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      float e0, e1;
+      f2_unpack(f2_add(z[i], shift), e0, e1);
+      const f32x2 e = f2_pack(exp2_approx(e0), exp2_approx(e1));
+      d[i] = f2_mul(e, CAP ? f2_fma(f2_mul(z[i], z[i]), bend2, gB2) : gB2);
+    }
+    store(Vec16<T>::round(d), v);
+  };
+  if (!live) {
+    for (int v = slice.v0 + tid; v < slice.v1; v += THREADS) store(make_uint4(0u, 0u, 0u, 0u), v);
+  } else if (small) {
+    dt_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) {
+      Vec16<T> a;
+      a.set(u);
+      f32x2 z[N / 2];
+      Z.template of<true, T>(a, z);
+      grad(z, v);
+    });
+  } else {
+#pragma unroll 1
+    for (int v = slice.v0 + tid; v < slice.v1; v += THREADS) {
+      Vec16<T> a;
+      a.set(__ldg(xv + v));
+      f32x2 z[N / 2];
+      Z.template of<false, T>(a, z);
+      grad(z, v);
+    }
   }
-  if (v < slice.v1) grad(__ldcs(xv + v), v);
-  for (int i = tid; i < slice.n_single(rank, blocks); i += DT_THREADS) {
+  for (int i = tid; i < singles; i += THREADS) {
     const int j = slice.single(i, rank);
     const float z = Z(to_float(x[j]));
     dx[j] = from_float<T>(live ? exp2_approx(z - lR) * (CAP ? fmaf(-bend * z, z, gB) : gB) : 0.f);
   }
   __syncthreads();   // the named tokens got the tail's gradient, too: theirs follows
-  const float l = s.l, W = s.W, flat = CAP ? 1.f / (Z.a * Z.a) : 0.f;
-  for (int k = tid; k < K; k += DT_THREADS) {
+  const float l = s.l, W = s.W;
+  for (int k = tid; k < K; k += THREADS) {
     const int id = en.id[k];
     if (id < 0 || !live) continue;
     const int o = slice.place(id);
@@ -325,7 +392,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_kernel(const xl_distill_pa
       for (int i = 0; i < K; ++i) pk += en.id[i] == id ? en.e[i] : 0.f;
     }
     const float z = en.z[k];
-    dx[id] = from_float<T>(g * (W * exp2_approx(z - l) - pk * s.pscale) * (CAP ? 1.f - flat * z * z : 1.f));
+    dx[id] = from_float<T>(g * (W * exp2_approx(z - l) - pk * s.pscale) * (CAP ? 1.f - Z.flat * z * z : 1.f));
   }
 }
 
@@ -349,7 +416,7 @@ static int dt_validate(const xl_distill_params* p) {
 // of at least 2048 tokens that exchange their sums through the cluster's shared memory.
 static int dt_blocks(int rows, int V) {
   int blocks = 1;
-  while (blocks < 8 && rows * (blocks * 2) <= 4 * 148 && V >= 2048 * (blocks * 2)) blocks *= 2;
+  while (blocks < DT_BLOCKS && rows * (blocks * 2) <= 4 * 148 && V >= 2048 * (blocks * 2)) blocks *= 2;
   return blocks;
 }
 
@@ -368,7 +435,7 @@ template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD> static int d
   attr[0].val.clusterDim = {(unsigned)blocks, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, *p, blocks));
+  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, *p, CappedZ<CAP>(p->cap, p->temperature), 1.0 / (double)p->temperature, blocks));
   return check_launch("xl_distill_topk");
 }
 

@@ -6,7 +6,7 @@
 
 namespace xl {
 
-constexpr int VOCAB_MAX = 1 << 19;   // longest row: sums of weights in 2^-44 stay below 2^63
+constexpr int VOCAB_MAX = 1 << 18;   // longest row: sums of weights in 2^-44 stay below 2^63
 constexpr int TOPK_MAX = 1024;       // teacher entries of a row
 
 // cap * tanh(x / cap) with quotient, tanh and product rounded to T each, as the reference's eager soft_cap does.
@@ -99,11 +99,16 @@ template <> struct Vec16<__nv_bfloat16> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[i] = f2_bits(w[i] << 16, w[i] & 0xffff0000u);
   }
-  __device__ __forceinline__ float largest() const {   // of the magnitudes; NaN does not count
+  // running largest magnitude (NaN does not count)
+  typedef __nv_bfloat162 Mag;
+  static __device__ __forceinline__ Mag no_mag() { return __float2bfloat162_rn(0.f); }
+  __device__ __forceinline__ Mag track(Mag m) const {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
-    const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
-    return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __hmax2(m, __habs2(h[i]));
+    return m;
   }
+  static __device__ __forceinline__ float largest(Mag m) { return __bfloat162float(__hmax(__low2bfloat16(m), __high2bfloat16(m))); }
   static __device__ __forceinline__ uint4 round(const f32x2 (&v)[4]) {
     uint32_t w[4];
 #pragma unroll
@@ -119,12 +124,15 @@ template <> struct Vec16<float> {
   static constexpr int N = 4;
   f32x2 p[2];
   __device__ __forceinline__ void set(const uint4& u) { p[0] = f2_bits(u.x, u.y); p[1] = f2_bits(u.z, u.w); }
-  __device__ __forceinline__ float largest() const {
+  typedef float Mag;
+  static __device__ __forceinline__ Mag no_mag() { return 0.f; }
+  __device__ __forceinline__ Mag track(Mag m) const {
     float a, b, c, d;
     f2_unpack(p[0], a, b);
     f2_unpack(p[1], c, d);
-    return fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d)));
+    return fmaxf(m, fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d))));
   }
+  static __device__ __forceinline__ float largest(Mag m) { return m; }
   static __device__ __forceinline__ uint4 round(const f32x2 (&v)[2]) {
     uint4 u;
     asm("mov.b64 {%0, %1}, %2;" : "=r"(u.x), "=r"(u.y) : "l"(v[0]));
@@ -135,35 +143,37 @@ template <> struct Vec16<float> {
 
 // z = a * tanh(x / cap) with a = cap log2(e) / T, or x * log2(e) / T without a cap: exponents of two.
 template <bool CAP> struct CappedZ {
-  float a, icap, c0, c1, c2, c3, c4, c5;
-  __device__ __forceinline__ CappedZ(float cap, float temperature) {
-    const double scale = 1.4426950408889634 / (double)temperature;
-    a = (float)(CAP ? scale * (double)cap : scale);
-    icap = CAP ? 1.f / cap : 0.f;
-    c0 = a; c1 = a * -0.33332958817481995f; c2 = a * 0.1332540661096573f; c3 = a * -0.05334443226456642f; c4 = a * 0.01958290860056877f;
-    c5 = a * -0.004716257099062204f;
+  float a, icap, flat;   // flat = 1 / a^2: the cap's slope is 1 - flat z^2
+  CappedZ(float cap, float temperature) {   // (on the host: the constants are kernel parameters)
+    const double scale = 1.4426950408889634 / (double)temperature, wide = CAP ? scale * (double)cap : scale;
+    a = (float)wide;
+    icap = CAP ? (float)(1.0 / (double)cap) : 0.f;
+    flat = CAP ? (float)(1.0 / (wide * wide)) : 0.f;
   }
+  static constexpr float C1 = -0.33332958817481995f, C2 = 0.1332540661096573f, C3 = -0.05334443226456642f, C4 = 0.01958290860056877f, C5 = -0.004716257099062204f;
   __device__ __forceinline__ float operator()(float x) const {
     if (!CAP) return x * a;
     const float z = x * icap, s = z * z;
     if (fabsf(z) > TANH_SMALL) return a * tanh_large(z);
-    return z * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, c5, c4), c3), c2), c1), c0);
+    return z * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, a * C5, a * C4), a * C3), a * C2), a * C1), a);
   }
-  template <typename T> __device__ __forceinline__ void of(const Vec16<T>& v, f32x2 (&out)[Vec16<T>::N / 2]) const {
+  __device__ __forceinline__ bool small(float magnitude) const { return !CAP || magnitude * icap <= TANH_SMALL; }
+  // of a vector's elements; SMALL: the caller has seen that all magnitudes are small
+  template <bool SMALL, typename T> __device__ __forceinline__ void of(const Vec16<T>& v, f32x2 (&out)[Vec16<T>::N / 2]) const {
     if (!CAP) {
 #pragma unroll
       for (int i = 0; i < Vec16<T>::N / 2; ++i) out[i] = f2_mul(v.p[i], f2_dup(a));
       return;
     }
-    if (v.largest() * icap <= TANH_SMALL) {
+    if (SMALL) {
 #pragma unroll
       for (int i = 0; i < Vec16<T>::N / 2; ++i) {
         const f32x2 z = f2_mul(v.p[i], f2_dup(icap)), s = f2_mul(z, z);
-        f32x2 q = f2_fma(s, f2_dup(c5), f2_dup(c4));
-        q = f2_fma(s, q, f2_dup(c3));
-        q = f2_fma(s, q, f2_dup(c2));
-        q = f2_fma(s, q, f2_dup(c1));
-        out[i] = f2_mul(z, f2_fma(s, q, f2_dup(c0)));
+        f32x2 q = f2_fma(s, f2_dup(a * C5), f2_dup(a * C4));
+        q = f2_fma(s, q, f2_dup(a * C3));
+        q = f2_fma(s, q, f2_dup(a * C2));
+        q = f2_fma(s, q, f2_dup(a * C1));
+        out[i] = f2_mul(z, f2_fma(s, q, f2_dup(a)));
       }
       return;
     }

@@ -9,7 +9,7 @@
 //
 // Precision.  The result is a whole number: a running sum that is off by d in relative terms picks another token with a
 // probability of up to d times the number of tokens.  Weights are therefore formed in 64 bits and summed as integers in
-// units of 2^-44 (rows are at most 2^19 long), which is exact and independent of the order of the atomics.
+// units of 2^-44 (rows are at most 2^18 long), which is exact and independent of the order of the atomics.
 #include "vocab_row.cuh"
 
 namespace xl {
