@@ -303,6 +303,33 @@ def test_distill_extremes(tag):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+def test_distill_rows_of_the_lowest_value(tag):
+    """The type's lowest value as a mask: of a whole row (its softmax is flat), of all but a few tokens, of the whole tail."""
+    import xlstm_b200
+    dt = DT[tag]
+    low = torch.finfo(dt).min
+    x = torch.full((3, 40), low).to(dt)
+    x[1, :10] = 1.0
+    x[2, :2] = 0.0
+    ids = torch.tensor([[0, 1]] * 3, dtype=torch.int32)
+    values = torch.zeros(3, 2)
+    for lse, want in ((None, [math.log(20.0), math.log(5.0), 0.0]), (torch.full((3,), math.log(2.0)), [math.log(20.0), math.log(5.0), 0.0])):
+        for T in (1.0, 0.5):
+            tl = None if lse is None else lse.cuda()
+            loss, grad = xlstm_b200.distill_topk_grad(x.cuda(), values.cuda(), ids.cuda(), None, None, T, tl)
+            n = 3 if lse is None else 2   # (float32(log 2) leaves 1 - 2 exp(-log 2) = 1.9e-9 to a tail at -3.4e38: the third loss is 6e29 or beyond)
+            assert (loss[:n].cpu() / T ** 2 - torch.tensor(want)[:n]).abs().max() < 1e-6
+            assert lse is None or float(loss[2]) > 1e29
+            flat = torch.zeros(3, 40)
+            flat[0], flat[1, :10], flat[2, :2] = 1 / 40, 1 / 10, 1 / 2
+            flat[:, :2] -= 0.5
+            assert (grad.float().cpu() / T - flat).abs().max() <= 2.0 ** -8 * 0.5
+            leaf = x.cuda().requires_grad_()
+            xlstm_b200.distill_topk(leaf, values.cuda(), ids.cuda(), None, T, tl).sum().backward()
+            assert torch.equal(leaf.grad, grad)
+
+
 def test_distill_masked_named_token_costs_infinity():
     import xlstm_b200
     x = torch.zeros(2, 8, device="cuda")

@@ -15,7 +15,7 @@ namespace xl {
 constexpr int DT_THREADS = 256, DT_WARPS = DT_THREADS / 32, DT_BLOCKS = 8;
 constexpr double DT_LN2 = 0.69314718055994530942;
 // what a row leaves for its gradient; the last two places hold a double
-enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_SMALL = 4, ST_TEACHER = 6 };
+enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_SMALL = 4, ST_REF = 5, ST_TEACHER = 6 };
 
 struct DtShared {
   double wd[3][DT_WARPS];
@@ -76,7 +76,8 @@ template <int STEP, typename F> __device__ __forceinline__ void dt_vectors(const
 __device__ __forceinline__ double dt_nanmax(double a, double b) { return a != a || b != b ? a + b : fmax(a, b); }   // (NaN survives)
 
 template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill_params p, const CappedZ<CAP> Z, const double invT, const int blocks) {
+__global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill_params p, const CappedZ<CAP> Z0, const double invT, const int blocks) {
+  CappedZ<CAP> Z = Z0;
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ DtShared s;
   constexpr int N = Vec16<T>::N, THREADS = DT_THREADS, WARPS = DT_WARPS;
@@ -103,6 +104,7 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
     return (en.bits[o >> 5] >> (o & 31)) & 1u;
   };
 
+  if (!LOSS && !CAP) Z.ref = st[ST_REF];
   // the teacher's entries, the student's logits there, and the bits of the tokens named
   if (LOSS) {
     for (int w = tid; w < (slice.end - slice.first + 31) / 32; w += THREADS) en.bits[w] = 0u;
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
   }
   const int with = min(WARPS, (K + 31) / 32);   // warps that have entries
   double m = -INFINITY;   // of t / T
-  float mS = -INFINITY;
+  float xS = -INFINITY;   // largest logit of the tokens named
   int any = 0, twice = 0, count = 0;
   if (warp < with) {
     for (int k = tid; k < K; k += THREADS) {
@@ -124,8 +126,9 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
       en.t[k] = t;
       any = 1;
       m = dt_nanmax(m, t);
-      en.z[k] = Z(to_float(x[id]));
-      mS = fmaxf(mS, en.z[k]);
+      const float xk = to_float(x[id]);
+      en.z[k] = LOSS && !CAP ? xk : Z(xk);   // (without a cap z waits for the row's largest)
+      xS = fmaxf(xS, xk);
       const int o = slice.place((int)id) - slice.first;
       if (LOSS && o >= 0 && o < slice.end - slice.first) {
         const int old = (atomicOr(&en.bits[o >> 5], 1u << (o & 31)) >> (o & 31)) & 1u;
@@ -137,12 +140,12 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         m = dt_nanmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (!BOUNDED) mS = fmaxf(mS, __shfl_xor_sync(0xffffffffu, mS, o));
+        if (!BOUNDED) xS = fmaxf(xS, __shfl_xor_sync(0xffffffffu, xS, o));
       }
       if (K >= V) count = __reduce_add_sync(0xffffffffu, count);
     }
     any = (__any_sync(0xffffffffu, any) ? 1 : 0) | (__any_sync(0xffffffffu, twice) ? 2 : 0);
-    if (lane == 0) { s.wd[2][warp] = m; s.wf[0][warp] = mS; s.wi[0][warp] = any; s.wi[1][warp] = count; }
+    if (lane == 0) { s.wd[2][warp] = m; s.wf[0][warp] = xS; s.wi[0][warp] = any; s.wi[1][warp] = count; }
   }
   __syncthreads();   // (the bits are there, too)
   any = 0;
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
   for (int w = 0; w < with; ++w) {
     if (LOSS) {
       m = dt_nanmax(m, s.wd[2][w]);
-      if (!BOUNDED) mS = fmaxf(mS, s.wf[0][w]);
+      if (!BOUNDED) xS = fmaxf(xS, s.wf[0][w]);
       count += s.wi[1][w];
     }
     any |= s.wi[0][w];
@@ -166,11 +169,40 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
     again = true;   // (not known here)
     L = *reinterpret_cast<const double*>(st + ST_TEACHER);
   }
-  mS = BOUNDED || mS == -INFINITY ? 0.f : mS;
+  float mR = 0.f, mS = 0.f;   // shifts of the two sums: their largest z (with a bounded z: none)
+  if (LOSS) {
+    __syncwarp();
+    if (blocks > 1) cluster_wait();
+    if (!BOUNDED) {
+      float xm = -INFINITY;
+      dt_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) {
+        Vec16<T> a;
+        a.set(u);
+        const unsigned int f = flags(v);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float x0, x1;
+          f2_unpack(a.p[i], x0, x1);
+          if (!(f >> (2 * i) & 1u)) xm = fmaxf(xm, x0);
+          if (!(f >> (2 * i + 1) & 1u)) xm = fmaxf(xm, x1);
+        }
+      });
+      for (int i = tid; i < singles; i += THREADS) {
+        const int j = slice.single(i, rank);
+        if (!flag(j)) xm = fmaxf(xm, to_float(x[j]));
+      }
+      xm = block_reduce<WARPS>(xm, OpMax(), s.wf[0]);
+      if (blocks > 1) xm = dt_exchange(xm, s.from[2], rank, blocks, OpMax());
+      Z.set_ref(fmaxf(xm, xS));
+      mR = xm == -INFINITY ? 0.f : fmaxf(Z(xm), -3e38f);   // (logits of the type's lowest value as masks: z = -inf)
+      mS = xS == -INFINITY ? 0.f : fmaxf(Z(xS), -3e38f);
+    }
+  }
   float sS = 0.f;   // of the slice's tokens named
   if (warp < with) {
     double E = 0.0, F = 0.0;   // sum of e_k, and of e_k (t_k - z_k)
     for (int k = tid; k < K; k += THREADS) {
+      if (LOSS && !CAP) en.z[k] = Z(en.z[k]);
       double e = 0.0;
       if (en.id[k] >= 0 && live) {
         e = exp(en.t[k] - L);
@@ -199,31 +231,6 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
 
   bool small = true;   // (this thread's) logits stay below three quarters of the cap
   if (LOSS) {
-    __syncwarp();
-    if (blocks > 1) cluster_wait();
-    float mR = 0.f;
-    if (!BOUNDED) {
-      float xm = -INFINITY;
-      dt_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) {
-        Vec16<T> a;
-        a.set(u);
-        const unsigned int f = flags(v);
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          float x0, x1;
-          f2_unpack(a.p[i], x0, x1);
-          if (!(f >> (2 * i) & 1u)) xm = fmaxf(xm, x0);
-          if (!(f >> (2 * i + 1) & 1u)) xm = fmaxf(xm, x1);
-        }
-      });
-      for (int i = tid; i < singles; i += THREADS) {
-        const int j = slice.single(i, rank);
-        if (!flag(j)) xm = fmaxf(xm, to_float(x[j]));
-      }
-      xm = block_reduce<WARPS>(xm, OpMax(), s.wf[0]);
-      if (blocks > 1) xm = dt_exchange(xm, s.from[2], rank, blocks, OpMax());
-      mR = xm == -INFINITY ? 0.f : Z(xm);
-    }
     // both sums over the slice.  The first try takes every magnitude for a small one and looks at the largest behind it;
     // a thread that met a large one sums its vectors again.
     float sR = 0.f;
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill
         if (rank == 0) {
           p.loss[row] = (float)((double)p.temperature * (double)p.temperature * loss);
           if (st) {
-            st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W; st[ST_SMALL] = all_small ? 1.f : 0.f;
+            st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W; st[ST_SMALL] = all_small ? 1.f : 0.f; st[ST_REF] = Z.ref;
             *reinterpret_cast<double*>(st + ST_TEACHER) = given ? L : L + lE * DT_LN2;
           }
         }

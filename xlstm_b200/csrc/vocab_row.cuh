@@ -141,28 +141,37 @@ template <> struct Vec16<float> {
   }
 };
 
-// z = a * tanh(x / cap) with a = cap log2(e) / T, or x * log2(e) / T without a cap: exponents of two.
+// z = a * tanh(x / cap) with a = cap log2(e) / T, or (x - ref) * log2(e) / T without a cap: exponents of two.  `ref` is a number
+// near the row's largest logit, so that rows near the type's lowest value (masks) do not overflow.
 template <bool CAP> struct CappedZ {
-  float a, icap, flat;   // flat = 1 / a^2: the cap's slope is 1 - flat z^2
+  float a, icap, ref, flat;   // flat = 1 / a^2: the cap's slope is 1 - flat z^2
   CappedZ(float cap, float temperature) {   // (on the host: the constants are kernel parameters)
     const double scale = 1.4426950408889634 / (double)temperature, wide = CAP ? scale * (double)cap : scale;
     a = (float)wide;
+    ref = 0.f;
     icap = CAP ? (float)(1.0 / (double)cap) : 0.f;
     flat = CAP ? (float)(1.0 / (wide * wide)) : 0.f;
   }
   static constexpr float C1 = -0.33332958817481995f, C2 = 0.1332540661096573f, C3 = -0.05334443226456642f, C4 = 0.01958290860056877f, C5 = -0.004716257099062204f;
   __device__ __forceinline__ float operator()(float x) const {
-    if (!CAP) return x * a;
+    if (!CAP) return (x - ref) * a;
     const float z = x * icap, s = z * z;
     if (fabsf(z) > TANH_SMALL) return a * tanh_large(z);
     return z * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, a * C5, a * C4), a * C3), a * C2), a * C1), a);
+  }
+  __device__ __forceinline__ void set_ref(float largest) { ref = fabsf(largest) <= 3.4028234e38f ? largest : 0.f; }   // (not of infinities)
+  // tanh(x / cap)
+  __device__ __forceinline__ float tanh_of(float x) const {
+    const float z = x * icap, s = z * z;
+    if (fabsf(z) > TANH_SMALL) return tanh_large(z);
+    return z * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, C5, C4), C3), C2), C1), 1.f);
   }
   __device__ __forceinline__ bool small(float magnitude) const { return !CAP || magnitude * icap <= TANH_SMALL; }
   // of a vector's elements; SMALL: the caller has seen that all magnitudes are small
   template <bool SMALL, typename T> __device__ __forceinline__ void of(const Vec16<T>& v, f32x2 (&out)[Vec16<T>::N / 2]) const {
     if (!CAP) {
 #pragma unroll
-      for (int i = 0; i < Vec16<T>::N / 2; ++i) out[i] = f2_mul(v.p[i], f2_dup(a));
+      for (int i = 0; i < Vec16<T>::N / 2; ++i) out[i] = f2_mul(f2_add(v.p[i], f2_dup(-ref)), f2_dup(a));
       return;
     }
     if (SMALL) {

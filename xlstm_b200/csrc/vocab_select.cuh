@@ -1,0 +1,309 @@
+// The largest logits of a row, sorted, without sorting the row.
+//
+// Mathematics.  Every thread keeps the largest logit of two groups of the row (the even and the odd places of its vectors).
+// If the k-th largest of the group maxima is t, at least k logits are >= t: t bounds the k-th largest logit from below, and with
+// G groups and k well below G only about -G ln(1 - k/G) logits reach it (71 for k = 64, G = 512).  So a first pass takes maxima, one
+// warp finds t by bisection over the leading 16 bits of the keys, a second pass collects what reaches t into a list, and only
+// the list is sorted, by (key, lower index).  Rows where too many logits reach t (crowds of equal ones, or all large logits in few
+// groups) are told by the length of the list, and left to the caller's exact selection.
+//
+// A row may be cut over a cluster of blocks: each finds the bound of its slice, the largest of the bounds holds for the row, and
+// block 0 gathers the lists through the cluster's shared memory.
+#pragma once
+
+#include "vocab_row.cuh"
+
+namespace xl {
+
+constexpr int SEL_CAP = 1024;      // entries of the list
+constexpr int SEL_BLOCKS = 8;
+constexpr int SEL_RANKED = 256;    // lists up to this length are sorted by counting who is larger
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+
+template <int THREADS> struct SelShared {
+  unsigned long long list[SEL_CAP];     // key (32 bits) and ~index
+  unsigned short group[2 * THREADS];    // leading 16 bits of the groups' largest keys
+  unsigned int from[2][SEL_BLOCKS];     // of the row's blocks: bound, largest key; written once a launch
+  unsigned int largest[THREADS / 32];
+  unsigned int n;                       // entries that reached the bound, also those beyond the list
+  unsigned int bound, top;              // leading 16 bits of the bound's key; key of the largest logit
+};
+
+template <typename T> __device__ __forceinline__ uint32_t list_key(T x) { return VocabKey<T>::of(x) << (32 - VocabKey<T>::BITS); }
+template <typename T> __device__ __forceinline__ float list_value(unsigned long long e) { return VocabKey<T>::value((uint32_t)(e >> 32) >> (32 - VocabKey<T>::BITS)); }
+
+// running maxima of the even and odd places of a thread's vectors; NaN does not count
+template <typename T> struct GroupMax;
+template <> struct GroupMax<__nv_bfloat16> {
+  __nv_bfloat162 m;
+  __device__ __forceinline__ GroupMax() : m(__float2bfloat162_rn(-INFINITY)) {}
+  __device__ __forceinline__ void add(const uint4& u) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    m = __hmax2(m, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  }
+  __device__ __forceinline__ void add_one(__nv_bfloat16 x) { m = __hmax2(m, __halves2bfloat162(x, __float2bfloat16(-INFINITY))); }
+  __device__ __forceinline__ float even() const { return __low2float(m); }
+  __device__ __forceinline__ float odd() const { return __high2float(m); }
+};
+template <> struct GroupMax<float> {
+  float a, b;
+  __device__ __forceinline__ GroupMax() : a(-INFINITY), b(-INFINITY) {}
+  __device__ __forceinline__ void add(const uint4& u) {
+    a = fmaxf(a, fmaxf(__uint_as_float(u.x), __uint_as_float(u.z)));
+    b = fmaxf(b, fmaxf(__uint_as_float(u.y), __uint_as_float(u.w)));
+  }
+  __device__ __forceinline__ void add_one(float x) { a = fmaxf(a, x); }
+  __device__ __forceinline__ float even() const { return a; }
+  __device__ __forceinline__ float odd() const { return b; }
+};
+
+// f(vector, its number) for v, v + STEP, .. below end, four loads under way at a time
+template <int STEP, typename F> __device__ __forceinline__ void for_vectors(const uint4* xv, int v, int end, F f) {
+#pragma unroll 1
+  for (; v + 3 * STEP < end; v += 4 * STEP) {
+    uint4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __ldg(xv + v + i * STEP);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f(u[i], v + i * STEP);
+  }
+#pragma unroll 1
+  for (; v < end; v += STEP) f(__ldg(xv + v), v);
+}
+
+template <typename T, int THREADS> struct Selector {
+  static constexpr int N = Vec16<T>::N;
+  SelShared<THREADS>& s;
+  const T* x;
+  RowSlice<T> slice;
+  int rank, blocks, singles;
+  const uint4* xv;
+
+  __device__ __forceinline__ Selector(SelShared<THREADS>& s_, const T* x_, int V, int rank_, int blocks_)
+      : s(s_), x(x_), slice(x_, V, rank_, blocks_), rank(rank_), blocks(blocks_) {
+    xv = reinterpret_cast<const uint4*>(x + slice.head);
+    singles = slice.n_single(rank, blocks);
+  }
+
+  // First pass: s.bound (a lower bound of the k-th largest) and s.top (the largest, NaN aside), both of the whole row.  Ends behind a
+  // barrier.
+  __device__ void bound(int k) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (blocks > 1) cluster_arrive();
+    GroupMax<T> g;
+    for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int) { g.add(u); });
+    for (int i = tid; i < singles; i += THREADS) g.add_one(x[slice.single(i, rank)]);
+    s.group[2 * tid] = (unsigned short)(key_of_float(g.even()) >> 16);
+    s.group[2 * tid + 1] = (unsigned short)(key_of_float(g.odd()) >> 16);
+    const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of_float(fmaxf(g.even(), g.odd())));
+    if (lane == 0) s.largest[tid >> 5] = mine;
+    if (tid == 0) s.n = 0u;
+    __syncthreads();
+    if (tid < 32) {
+      constexpr int PER = 2 * THREADS / 64;   // pairs a lane
+      const uint32_t* two = reinterpret_cast<const uint32_t*>(s.group);
+      uint32_t key[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) key[i] = two[i * 32 + lane];
+      const uint32_t top = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s.largest[lane] : 0u);
+      uint32_t t = 0u;
+      for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+        const uint32_t c = t | bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) n += (key[i] >> 16 >= c) + ((key[i] & 0xffffu) >= c);
+        if (__reduce_add_sync(0xffffffffu, n) >= k) t = c;
+      }
+      if (blocks > 1) {
+        __syncwarp();
+        cluster_wait();
+        if (lane < blocks) {
+          st_cluster_u32(mapa_u32(smem_u32(&s.from[0][rank]), lane), t);
+          st_cluster_u32(mapa_u32(smem_u32(&s.from[1][rank]), lane), top);
+        }
+      } else if (lane == 0) {
+        s.bound = t;
+        s.top = top;
+      }
+    }
+    if (blocks > 1) {
+      if (tid >= 32) cluster_wait();
+      __syncwarp();
+      cluster_sync_all();
+      if (tid == 0) {
+        uint32_t t = 0u, top = 0u;
+        for (int r = 0; r < blocks; ++r) { t = max(t, s.from[0][r]); top = max(top, s.from[1][r]); }
+        s.bound = t;
+        s.top = top;
+      }
+    }
+    __syncthreads();
+  }
+
+  // the bound as a number; -inf where there are too few groups for one
+  __device__ __forceinline__ float least() const {
+    return s.bound == 0u ? -INFINITY : VocabKey<T>::value(s.bound << (VocabKey<T>::BITS - 16));
+  }
+
+  // Second pass over the slice: what reaches `least` into the list; `also(vector, number)` and `also_one(element)` see everything.
+  template <typename F, typename G> __device__ void collect(float least, F also, G also_one) {
+    const int tid = threadIdx.x;
+    auto take = [&](T e, int j) {
+      if (to_float(e) >= least && *const_cast<volatile unsigned int*>(&s.n) <= SEL_CAP) {   // (a crowd need not be counted)
+        const unsigned int at = atomicAdd(&s.n, 1u);
+        if (at < SEL_CAP) s.list[at] = (unsigned long long)list_key(e) << 32 | (uint32_t)~j;
+      }
+    };
+    for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) {
+      also(u, v);
+      GroupMax<T> g;
+      g.add(u);
+      if (fmaxf(g.even(), g.odd()) >= least) {
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < N; ++i) take(e[i], slice.element(v) + i);
+      }
+    });
+    for (int i = tid; i < singles; i += THREADS) {
+      const int j = slice.single(i, rank);
+      also_one(x[j]);
+      take(x[j], j);
+    }
+  }
+
+  // Behind a barrier of the block (and of the cluster): all lists of the row in block 0's.  Returns the row's number of entries there
+  // (above SEL_CAP: too many).  Every block has to come here; the others are done then.
+  __device__ unsigned int gather() {
+    if (blocks == 1) return s.n;
+    cluster_sync_all();
+    unsigned int n = s.n;
+    if (rank == 0) {
+      for (int r = 1; r < blocks; ++r) {
+        const unsigned int more = ld_cluster_u32(mapa_u32(smem_u32(&s.n), r));
+        const uint32_t from = mapa_u32(smem_u32(s.list), r);
+        for (unsigned int i = threadIdx.x; i < min(more, (unsigned int)SEL_CAP) && n + i < SEL_CAP; i += THREADS) s.list[n + i] = ld_cluster_u64(from + 8 * i);
+        n += more;
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    return n;
+  }
+};
+
+// The exact selection, for rows that the bound does not thin out: the k <= SEL_CAP largest of the row into `list`, in any order,
+// by a histogram of the leading 11 bits of the keys, one of the next bits inside the bin of the k-th, and so on.  NaN counts as
+// the smallest.  One block; ends behind a barrier.
+constexpr int SEL_BINS = 2048;
+template <int THREADS> struct SelExact {
+  unsigned int count[SEL_BINS];
+  unsigned int wc[THREADS / 32], bin, above, n;
+};
+template <typename T, int THREADS> __device__ __noinline__ void select_exact(SelExact<THREADS>& s, unsigned long long* list, const T* x, int V, int k) {
+  constexpr int BITS = VocabKey<T>::BITS, WARPS = THREADS / 32, PER = SEL_BINS / THREADS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t prefix = 0u;
+  unsigned int want = (unsigned int)k;   // of those that share the prefix
+  for (int left = BITS; left > 0;) {
+    const int step = left > 11 ? 11 : left, bins = 1 << step;
+    __syncthreads();
+    for (int b = tid; b < bins; b += THREADS) s.count[b] = 0u;
+    __syncthreads();
+    for (int j = tid; j < V; j += THREADS) {
+      const uint32_t key = VocabKey<T>::of(x[j]);
+      if (left < BITS && key >> left != prefix) continue;
+      atomicAdd(&s.count[(key >> (left - step)) & (uint32_t)(bins - 1)], 1u);
+    }
+    __syncthreads();
+    const int b0 = bins - 1 - PER * tid;   // PER bins a thread, from the top
+    unsigned int sum = 0u;
+    for (int i = 0; i < PER; ++i) sum += b0 - i >= 0 ? s.count[b0 - i] : 0u;
+    unsigned int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) s.wc[warp] = upto;
+    __syncthreads();
+    unsigned int before = upto - sum;
+    for (int w = 0; w < warp; ++w) before += s.wc[w];
+    for (int i = 0; i < PER; ++i) {
+      const unsigned int c = b0 - i >= 0 ? s.count[b0 - i] : 0u;
+      if (before < want && want <= before + c) { s.bin = (unsigned int)(b0 - i); s.above = before; }
+      before += c;
+    }
+    __syncthreads();
+    prefix = (prefix << step) | s.bin;
+    want -= s.above;
+    left -= step;
+  }
+  // the tokens above it, in any order, then the first `want` of its equals in index order (every warp takes a stretch)
+  if (tid == 0) s.n = 0u;
+  const int per = (V + WARPS - 1) / WARPS, j0 = min(V, warp * per), j1 = min(V, j0 + per);
+  __syncthreads();
+  auto entry = [](uint32_t key, int j) { return (unsigned long long)(key << (32 - BITS)) << 32 | (uint32_t)~j; };
+  unsigned int n = 0u;
+  for (int j = j0 + lane; j < j1; j += 32) {
+    const uint32_t key = VocabKey<T>::of(x[j]);
+    if (key > prefix) list[atomicAdd(&s.n, 1u)] = entry(key, j);
+    n += key == prefix;
+  }
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (lane == 0) s.wc[warp] = n;
+  __syncthreads();
+  unsigned int before = 0u;
+  for (int w = 0; w < warp; ++w) before += s.wc[w];
+  if (n > 0u && before < want)
+    for (int j = j0; j < j1 && before < want; j += 32) {
+      const bool hit = j + lane < j1 && VocabKey<T>::of(x[j + lane]) == prefix;
+      const unsigned int mask = __ballot_sync(0xffffffffu, hit), mine = before + __popc(mask & ((1u << lane) - 1u));
+      if (hit && mine < want) list[k - want + mine] = entry(prefix, j + lane);
+      before += __popc(mask);
+    }
+  __syncthreads();
+}
+
+// Descending sort of the n <= SEL_CAP entries (all different); ends behind a barrier.
+template <int THREADS> __device__ void sort_list(unsigned long long* list, int n) {
+  const int tid = threadIdx.x;
+  if (n <= SEL_RANKED && n <= THREADS) {
+    const unsigned long long mine = tid < n ? list[tid] : 0ull;
+    int above = 0;
+    if ((tid & ~31) < n) {
+      int i = 0;
+      for (; i + 4 <= n; i += 4) above += (list[i] > mine) + (list[i + 1] > mine) + (list[i + 2] > mine) + (list[i + 3] > mine);
+      for (; i < n; ++i) above += list[i] > mine;
+    }
+    __syncthreads();
+    if (tid < n) list[above] = mine;
+    __syncthreads();
+    return;
+  }
+  int size = 1;
+  while (size < n) size <<= 1;
+  for (int i = n + tid; i < size; i += THREADS) list[i] = 0ull;
+  __syncthreads();
+  for (int len = 2; len <= size; len <<= 1)
+    for (int step = len >> 1; step > 0; step >>= 1) {
+      for (int i = tid; i < size / 2; i += THREADS) {
+        const int a = 2 * i - (i & (step - 1)), b = a + step;
+        const unsigned long long u = list[a], v = list[b];
+        if ((u < v) == ((a & len) == 0)) { list[a] = v; list[b] = u; }
+      }
+      __syncthreads();
+    }
+}
+
+}  // namespace xl
