@@ -24,57 +24,79 @@ constexpr int VS_VALUES = 4096;   // distinct bf16 values of a row that the coun
 constexpr double VS_ONE = 17592186044416.0;   // 2^44
 typedef unsigned long long u64;
 
-// e^x for x <= 0: 2^n times the Taylor series of 2^f, |f| <= 1/2, to degree 13 (relative error 3e-16)
-__device__ __forceinline__ double vs_exp(double x) {
-  const double t = fmax(x, -700.0) * 1.4426950408889634, n = rint(t);
-  const double f = fma(fmax(x, -700.0), 1.4426950408889634, -n);
-  double p = 1.3691488853904128e-12;
-  p = fma(p, f, 2.5678435993488206e-11);
-  p = fma(p, f, 4.4455382718708116e-10);
-  p = fma(p, f, 7.054911620801123e-09);
-  p = fma(p, f, 1.01780860092397e-07);
-  p = fma(p, f, 1.321548679014431e-06);
-  p = fma(p, f, 1.5252733804059841e-05);
-  p = fma(p, f, 0.0001540353039338161);
-  p = fma(p, f, 0.0013333558146428443);
-  p = fma(p, f, 0.009618129107628477);
-  p = fma(p, f, 0.05550410866482158);
-  p = fma(p, f, 0.24022650695910072);
-  p = fma(p, f, 0.6931471805599453);
-  p = fma(p, f, 1.0);
-  return __hiloint2double(__double2hiint(p) + ((int)n << 20), __double2loint(p));   // (n >= -1010: no subnormal)
+// Conversions between 64-bit numbers and integers or fp32 go through the slowest unit of the SM; here they are bit moves and
+// additions of powers of two.
+__device__ __forceinline__ double vs_double(float v) {   // (what is below 2^-126 counts as 0)
+  const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
+  return m < 0x00800000u ? 0.0 : __hiloint2double((int)((b & 0x80000000u) | ((m >> 3) + 0x38000000u)), (int)(m << 29));
 }
-// 1 / d, 1 <= d <= 2: two Newton steps from the fp32 reciprocal
+__device__ __forceinline__ u64 vs_whole(double w) {   // rint(w 2^44), 0 <= w <= 1
+  return (u64)__double_as_longlong(fma(w, VS_ONE, 4503599627370496.0)) & 0x000fffffffffffffull;
+}
+__device__ __forceinline__ double vs_number(u64 m) {   // m < 2^63
+  return fma((double)(int)(m >> 32), 4294967296.0, (double)(uint32_t)m);
+}
+
+// e^x for x <= 0: 2^n times the Taylor series of 2^f, |f| <= 1/2, to degree 10: relative error 3e-13, a tenth of the unit of the sums
+__device__ __forceinline__ double vs_exp(double x) {
+  constexpr double LOG2E_64 = 1.4426950408889634, ROUND = 6755399441055744.0;   // 1.5 * 2^52: adding it rounds to whole numbers
+  x = x > -700.0 ? x : -700.0;
+  const double r = fma(x, LOG2E_64, ROUND), f = fma(x, LOG2E_64, ROUND - r);
+  const double f2 = f * f, f4 = f2 * f2;   // (in halves of halves: a chain of five instead of ten)
+  const double p0 = fma(fma(0.05550410866482158, f, 0.24022650695910072), f2, fma(0.6931471805599453, f, 1.0));
+  const double p1 = fma(fma(1.5252733804059841e-05, f, 0.0001540353039338161), f2, fma(0.0013333558146428443, f, 0.009618129107628477));
+  const double p2 = fma(7.054911620801123e-09, f2, fma(1.01780860092397e-07, f, 1.321548679014431e-06));
+  const double p = fma(fma(p2, f4, p1), f4, p0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20), __double2loint(p));   // (exponent >= -1010: no subnormal)
+}
+// 1 / d, 1 <= d <= 2: a Newton step from the fp32 reciprocal (2^-22 squared)
 __device__ __forceinline__ double vs_inverse(double d) {
-  double r = (double)__frcp_rn((float)d);
-  r = fma(r, fma(-d, r, 1.0), r);
+  const uint32_t hi = (uint32_t)__double2hiint(d), lo = (uint32_t)__double2loint(d);
+  const float f = hi >= 0x40000000u ? 2.f : __uint_as_float(0x3f800000u | (hi & 0x000fffffu) << 3 | lo >> 29);
+  const double r = vs_double(__fdividef(1.f, f));
   return fma(r, fma(-d, r, 1.0), r);
 }
 
 // what a row's tokens weigh
-template <typename T> struct VsWeights {
+struct VsWeights {
   double cap, icap, ymax, invT;
-  uint32_t kmax;
-  __device__ __forceinline__ void set(float cap_, float temperature, float largest) {
-    cap = cap_;
-    icap = cap_ > 0.f ? 1.0 / (double)cap_ : 0.0;
-    invT = 1.0 / (double)temperature;
-    kmax = VocabKey<T>::of(from_float<T>(largest));
-    ymax = capped(largest);
-  }
+  float largest;
   __device__ __forceinline__ double capped(float v) const {
-    if (!(cap > 0.0)) return v;
-    const double e = vs_exp(-2.0 * fabs((double)v) * icap);
-    return copysign(cap * (1.0 - e) * vs_inverse(1.0 + e), (double)v);
+    if (!(cap > 0.0)) return (double)v;
+    const double e = vs_exp(-2.0 * vs_double(fabsf(v)) * icap);
+    const double y = cap * (1.0 - e) * vs_inverse(1.0 + e);
+    return v < 0.f ? -y : y;
   }
-  __device__ __forceinline__ double of(uint32_t key) const {
-    if (key == kmax) return 1.0;
-    const float v = VocabKey<T>::value(key);
-    if (!(v > -INFINITY) || ymax == INFINITY) return 0.0;   // NaN and -inf; next to +inf
-    return vs_exp(fmin((capped(v) - ymax) * invT, 0.0));
+  __device__ __forceinline__ void set(double cap_, double icap_, double invT_, float largest_) {
+    cap = cap_;
+    icap = icap_;
+    invT = invT_;
+    largest = largest_;
+    ymax = capped(largest_);
   }
-  static __device__ __forceinline__ u64 whole(double w) { return __double2ull_rn(w * VS_ONE); }
+  __device__ __forceinline__ double of(float v, double y) const {
+    const double w = vs_exp((y - ymax) * invT);
+    return v == largest ? 1.0 : !(v > -INFINITY) || largest == INFINITY ? 0.0 : w;   // 0: NaN and -inf; next to +inf
+  }
+  __device__ __forceinline__ double of(float v) const { return of(v, capped(v)); }
+  // several at a time: a 64-bit instruction's result takes some forty cycles
+  template <int M> __device__ __forceinline__ void of(const float (&v)[M], double (&out)[M]) const {
+    double y[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) y[i] = capped(v[i]);
+#pragma unroll
+    for (int i = 0; i < M; ++i) out[i] = of(v[i], y[i]);
+  }
+  static __device__ __forceinline__ u64 whole(double w) { return vs_whole(w); }
 };
+
+// ceil(sum / each), at most 2^18: the fp32 quotient is off by one at most
+__device__ __forceinline__ unsigned int vs_steps(u64 sum, u64 each) {
+  unsigned int q = (unsigned int)((float)sum / (float)each);
+  while ((u64)q * each < sum) ++q;
+  while (q > 0u && (u64)(q - 1u) * each >= sum) --q;
+  return q;
+}
 
 struct VsPlace {
   uint32_t key;        // key of the token found
@@ -95,10 +117,10 @@ struct VsSettings {
     u = p.u[row];
   }
   // the running mass that top_p asks for; at most 1 (in units): the first token alone
-  __device__ __forceinline__ double top_p_goal(u64 kept) const { return ceil((double)top_p * (double)kept); }
+  __device__ __forceinline__ double top_p_goal(u64 kept) const { return ceil((double)top_p * vs_number(kept)); }
   // and the one that u asks for
   __device__ __forceinline__ u64 goal(u64 kept) const {
-    const double at = (double)u * (double)kept;
+    const double at = (double)u * vs_number(kept);
     return min(kept, at > 0.0 ? (u64)at + 1ull : 1ull);   // (NaN: the first)
   }
 };
@@ -158,7 +180,7 @@ template <typename T, int THREADS> struct VsRow {
   VsScan<THREADS>& scan;
   const T* x;
   int V;
-  VsWeights<T> w;
+  VsWeights w;
 
   // one prefix question over a histogram: the bin, from the top, in which the running count (or mass) reaches `goal`
   __device__ void find(const VsHist& h, int bins, bool by_mass, u64 goal, unsigned int base_cnt, u64 base_mass) {
@@ -191,7 +213,7 @@ template <typename T, int THREADS> struct VsRow {
       if (left < VocabKey<T>::BITS && key >> left != prefix) continue;
       const uint32_t b = (key >> (left - step)) & (uint32_t)(bins - 1);
       atomicAdd(&h.count[b], 1u);
-      const u64 m = VsWeights<T>::whole(w.of(key));
+      const u64 m = VsWeights::whole(w.of(VocabKey<T>::value(key)));
       if (m) atomicAdd(&h.mass[b], m);
     }
     __syncthreads();
@@ -214,7 +236,7 @@ template <typename T, int THREADS> struct VsRow {
     const u64 each = s.bin_mass / s.cnt;   // of every token of this key
     VsPlace r;
     r.key = prefix;
-    r.rank = by_mass ? (unsigned int)((goal - s.base_mass + each - 1) / each) - 1u : (unsigned int)(goal - s.base_cnt) - 1u;
+    r.rank = by_mass ? vs_steps(goal - s.base_mass, each) - 1u : (unsigned int)(goal - s.base_cnt) - 1u;
     r.upto = s.base_mass + (u64)(r.rank + 1u) * each;
     __syncthreads();
     return r;
@@ -229,8 +251,8 @@ template <typename T, int THREADS> struct VsRow {
     for (int b = threadIdx.x; b < VS_BINS; b += THREADS) all += s.top.mass[b];
     if (set.min_p > 0.f)
       for (int j = threadIdx.x; j < V; j += THREADS) {
-        const double v = w.of(VocabKey<T>::of(x[j]));
-        if (v >= (double)set.min_p) over += VsWeights<T>::whole(v);
+        const double v = w.of(to_float(x[j]));
+        if (v >= (double)set.min_p) over += VsWeights::whole(v);
       }
     vs_scan<THREADS>(scan, none, all, &tc, &t);
     u64 kept = t;
@@ -251,26 +273,49 @@ template <typename T, int THREADS> struct VsRow {
 
 // ---------------------------------------------------------------------------------------------- counts (bf16)
 struct VsCounts {
-  unsigned int pair[32768];          // counters of the patterns 2 i and 2 i + 1
+  union {
+    unsigned int pair[32768];        // counters of the patterns 2 i and 2 i + 1
+    u64 each[VS_VALUES];             // when the values have been listed: the weight of a token of each
+  };
   unsigned int value[VS_VALUES];     // pattern << 16 | count, in order of descending value
-  unsigned int bits, cnt, base_cnt;
-  u64 base_mass, each;
+  unsigned int group[256];           // non-empty bins of 256 patterns each, in that order; then those in front
+  unsigned int values, counted;
+  VsPlace place;
 };
 
-// The pattern of rank-th value of a block of 64: blocks 511 .. 0 of positive patterns from the top, then 512 .. 1023 of negative ones.
-// false: too many values, or a counter ran over (then they do not sum up to V).
-template <int THREADS> __device__ bool vs_counts(VsCounts& s, VsScan<THREADS>& scan, const __nv_bfloat16* x, int V, int* values) {
-  static_assert(THREADS == 1024, "a block of 64 patterns per thread");
-  const int tid = threadIdx.x, lane = tid & 31;
+// The row's values in order.  Units of eight patterns (16 bytes) come in the order of descending value: the positive ones
+// from the top, then the negative ones; 32 units are a group, and the groups go round the warps, since most of a row's
+// values sit side by side.  false: too many values, or a counter ran over 65 535 (then they do not sum up to V).
+template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat16* x, int V) {
+  constexpr int WARPS = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // (eight loads a thread are under way while the counters are cleared: the whole of a row of up to 65 536)
+  constexpr int BATCH = 8;
+  const RowSlice<__nv_bfloat16> slice(x, V, 0, 1);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + slice.head);
+  uint4 u[BATCH];
+  auto load = [&](int v) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      if (v + i * THREADS < slice.vectors) u[i] = __ldg(xv + v + i * THREADS);
+  };
+  load(tid);
   for (int i = tid; i < 8192; i += THREADS) reinterpret_cast<uint4*>(s.pair)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid == 0) s.counted = 0u;
   __syncthreads();
   auto count = [&](uint32_t bits) { atomicAdd(&s.pair[bits >> 1], bits & 1u ? 0x10000u : 1u); };
-  const RowSlice<__nv_bfloat16> slice(x, V, 0, 1);
-  for_vectors<THREADS>(reinterpret_cast<const uint4*>(x + slice.head), tid, slice.vectors, [&](const uint4& u, int) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll 1
+  for (int v = tid; v < slice.vectors;) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { count(w[i] & 0xffffu); count(w[i] >> 16); }
-  });
+    for (int i = 0; i < BATCH; ++i)
+      if (v + i * THREADS < slice.vectors) {
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) { count(w[h] & 0xffffu); count(w[h] >> 16); }
+      }
+    v += BATCH * THREADS;
+    load(v);
+  }
   for (int i = tid; i < slice.n_single(0, 1); i += THREADS) count(__bfloat16_as_ushort(x[slice.single(i, 0)]));
   __syncthreads();
   if (tid == 0) {   // -0 goes with +0
@@ -279,81 +324,127 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, VsScan<THREADS>& s
     s.pair[0] += minus;
   }
   __syncthreads();
-  const bool positive = tid < 512;
-  const int block = positive ? 511 - tid : tid;   // of 64 patterns
-  const unsigned int* words = s.pair + 32 * block;
-  const int first_nan = block == 510 || block == 1022 ? 1 : block == 511 || block == 1023 ? 0 : 64;   // (inf is pattern 0 of block 510)
-  u64 mask = 0ull;
-  unsigned int sum = 0u;
-  for (int i = 0; i < 32; ++i) {   // (each lane starts at another word: another bank)
-    const int at = (i + lane) & 31;
-    const unsigned int w = words[at], lo = w & 0xffffu, hi = w >> 16;
-    sum += lo + hi;
-    if (2 * at < first_nan && lo) mask |= 1ull << (2 * at);
-    if (2 * at + 1 < first_nan && hi) mask |= 2ull << (2 * at);
-  }
-  unsigned int n = (unsigned int)__popcll(mask), total;
-  u64 counted = sum, all;
-  vs_scan<THREADS>(scan, n, counted, &total, &all);
-  *values = (int)total;
-  if (all != (u64)V || total > VS_VALUES) return false;
-  for (int i = 0; i < 32; ++i) {
-    const int at = (i + lane) & 31;
-    const unsigned int w = words[at];
+  const uint4* units = reinterpret_cast<const uint4*>(s.pair);
+  auto unit_of = [&](int g) { return g < 128 ? 4095 - (g * 32 + lane) : g * 32 + lane; };
+  // a unit's non-empty bins as bits, NaN (patterns above infinity, which starts the units 0xff0 and 0x1ff0) aside
+  auto filled = [](const uint4& u, int unit) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    unsigned int m = 0u;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int b = 2 * at + h;
-      if (!(mask >> b & 1ull)) continue;
-      const unsigned int front = positive ? (unsigned int)__popcll(mask >> b) - 1u : (unsigned int)__popcll(mask & ((1ull << b) - 1ull));
-      s.value[n + front] = (uint32_t)(64 * block + b) << 16 | (h ? w >> 16 : w & 0xffffu);
+    for (int i = 0; i < 4; ++i) m |= (w[i] & 0xffffu ? 1u : 0u) << (2 * i) | (w[i] >> 16 ? 2u : 0u) << (2 * i);
+    const int in_sign = unit & 0xfff;
+    return in_sign < 0xff0 ? m : in_sign == 0xff0 ? m & 1u : 0u;
+  };
+  constexpr int ROUNDS = 256 / WARPS;
+  uint4 mine[ROUNDS];   // (a thread's units stay in registers for the second look)
+  unsigned int sum = 0u;
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) mine[i] = units[unit_of(i * WARPS + warp)];
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const uint4 u = mine[i];
+    unsigned int n = 0u;
+    if (__any_sync(0xffffffffu, (u.x | u.y | u.z | u.w) != 0u)) {
+      n = __reduce_add_sync(0xffffffffu, __popc(filled(u, unit_of(i * WARPS + warp))));
+      sum += (u.x & 0xffffu) + (u.x >> 16) + (u.y & 0xffffu) + (u.y >> 16) + (u.z & 0xffffu) + (u.z >> 16) + (u.w & 0xffffu) + (u.w >> 16);
     }
+    if (lane == 0) s.group[i * WARPS + warp] = n;
+  }
+  if (V > 65535) {
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) atomicAdd(&s.counted, sum);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    unsigned int c[8], n = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n += c[i] = s.group[8 * lane + i];
+    unsigned int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) s.values = upto;
+    upto -= n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { s.group[8 * lane + i] = upto; upto += c[i]; }
+  }
+  __syncthreads();
+  if ((V > 65535 && s.counted != (unsigned int)V) || s.values > VS_VALUES) return false;
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int g = i * WARPS + warp, unit = unit_of(g);
+    const uint4 u = mine[i];
+    if (!__any_sync(0xffffffffu, (u.x | u.y | u.z | u.w) != 0u)) continue;
+    const unsigned int m = filled(u, unit), n = __popc(m);
+    unsigned int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    unsigned int* out = s.value + s.group[g] + upto - n;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int b = 0; b < 8; ++b)
+      if (m >> b & 1u) {
+        const unsigned int front = g < 128 ? __popc(m >> b) - 1u : __popc(m & ((1u << b) - 1u));
+        out[front] = (uint32_t)(8 * unit + b) << 16 | (w[b >> 1] >> (16 * (b & 1)) & 0xffffu);
+      }
   }
   __syncthreads();
   return true;
 }
 
 template <int THREADS>
-__device__ VsPlace vs_counted_sample(VsCounts& s, VsScan<THREADS>& scan, const VsWeights<__nv_bfloat16>& w, const VsSettings& set, int values, int V) {
-  constexpr int PER = VS_VALUES / THREADS;
-  const int tid = threadIdx.x, per = (values + THREADS - 1) / THREADS, i0 = min(values, tid * per);
+__device__ VsPlace vs_counted_sample(VsCounts& s, VsScan<THREADS>& scan, const VsWeights& w, const VsSettings& set) {
+  const int tid = threadIdx.x, values = (int)s.values, per = (values + THREADS - 1) / THREADS, i0 = min(values, tid * per), i1 = min(values, i0 + per);
   auto key_of = [](uint32_t e) { return VocabKey<__nv_bfloat16>::of(__ushort_as_bfloat16((unsigned short)(e >> 16))); };
-  u64 each[PER], mass = 0ull, over = 0ull, all, t;
-  unsigned int cnt[PER], count = 0u, tc;
+  u64 over = 0ull, mass = 0ull, all, t;
+  unsigned int count = 0u, tc;
+#pragma unroll 1
+  for (int i = tid; i < values; i += 3 * THREADS) {
+    uint32_t e[3];
+    float x[3];
+    double v[3];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    each[i] = 0ull;
-    cnt[i] = 0u;
-    if (i < per && i0 + i < values) {
-      const uint32_t e = s.value[i0 + i];
-      const double v = w.of(key_of(e));
-      each[i] = VsWeights<__nv_bfloat16>::whole(v);
-      cnt[i] = e & 0xffffu;
-      mass += each[i] * cnt[i];
-      count += cnt[i];
-      if (v >= (double)set.min_p) over += each[i] * cnt[i];
-    }
+    for (int h = 0; h < 3; ++h) { e[h] = s.value[min(i + h * THREADS, values - 1)]; x[h] = __uint_as_float(e[h] & 0xffff0000u); }
+    w.of(x, v);
+#pragma unroll
+    for (int h = 0; h < 3; ++h)
+      if (i + h * THREADS < values) {
+        const u64 each = VsWeights::whole(v[h]);
+        s.each[i + h * THREADS] = each;
+        if (v[h] >= (double)set.min_p) over += each * (e[h] & 0xffffu);
+      }
   }
+  __syncthreads();
+  for (int i = i0; i < i1; ++i) { const unsigned int c = s.value[i] & 0xffffu; mass += s.each[i] * c; count += c; }
   u64 before_m = mass;
   unsigned int before_c = count;
   vs_scan<THREADS>(scan, before_c, before_m, &tc, &all);
+  // (the thread that has the place works it out)
   auto find = [&](bool by_mass, u64 goal) {
-    u64 m = before_m;
-    unsigned int c = before_c;
-    const u64 lo = by_mass ? m : c, hi = lo + (by_mass ? mass : count);
+    const u64 lo = by_mass ? before_m : before_c, hi = lo + (by_mass ? mass : count);
     if (lo < goal && goal <= hi) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const u64 bm = each[i] * cnt[i], b = by_mass ? m : c, e = b + (by_mass ? bm : cnt[i]);
-        if (b < goal && goal <= e) { s.bits = s.value[i0 + i] >> 16; s.cnt = cnt[i]; s.base_cnt = c; s.base_mass = m; s.each = each[i]; }
+      u64 m = before_m;
+      unsigned int c = before_c;
+      for (int i = i0;; ++i) {
+        const unsigned int bc = s.value[i] & 0xffffu;
+        const u64 each = s.each[i], bm = each * bc;
+        if (goal <= (by_mass ? m + bm : (u64)(c + bc))) {
+          s.place.key = key_of(s.value[i]);
+          s.place.rank = by_mass ? vs_steps(goal - m, each) - 1u : (unsigned int)(goal - c) - 1u;
+          s.place.upto = m + (u64)(s.place.rank + 1u) * each;
+          break;
+        }
         m += bm;
-        c += cnt[i];
+        c += bc;
       }
     }
     __syncthreads();
-    VsPlace r;
-    r.key = key_of(s.bits << 16);
-    r.rank = by_mass ? (unsigned int)((goal - s.base_mass + s.each - 1) / s.each) - 1u : (unsigned int)(goal - s.base_cnt) - 1u;
-    r.upto = s.base_mass + (u64)(r.rank + 1u) * s.each;
+    const VsPlace r = s.place;
     __syncthreads();
     return r;
   };
@@ -373,61 +464,80 @@ __device__ VsPlace vs_counted_sample(VsCounts& s, VsScan<THREADS>& scan, const V
   return find(true, set.goal(kept));
 }
 
-// index of the token of key `key` that has `rank` others in front of it; every warp takes a stretch of the row
+// places of a vector's elements that equal v, as bits (-0 equals +0)
+template <typename T> __device__ __forceinline__ unsigned int vs_equal(const uint4& u, T v);
+template <> __device__ __forceinline__ unsigned int vs_equal<__nv_bfloat16>(const uint4& u, __nv_bfloat16 v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 two = __halves2bfloat162(v, v);
+  unsigned int m = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m |= (__heq2_mask(h[i], two) & 0x00020001u) << (2 * i);   // bits 2 i and 2 i + 17
+  return (m | m >> 16) & 0xffu;
+}
+template <> __device__ __forceinline__ unsigned int vs_equal<float>(const uint4& u, float v) {
+  return (__uint_as_float(u.x) == v ? 1u : 0u) | (__uint_as_float(u.y) == v ? 2u : 0u) | (__uint_as_float(u.z) == v ? 4u : 0u) | (__uint_as_float(u.w) == v ? 8u : 0u);
+}
+
+// index of the token of key `key` (a number's) that has `rank` others in front of it; every warp takes a stretch of the row
 template <typename T, int THREADS> __device__ void vs_locate(unsigned int* wc, const T* x, int V, uint32_t key, unsigned int rank, int64_t* out) {
-  constexpr int WARPS = THREADS / 32, N = Vec16<T>::N;
+  constexpr int WARPS = THREADS / 32, KEEP = 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T value = from_float<T>(VocabKey<T>::value(key));
+  const float number = to_float(value);
   const RowSlice<T> slice(x, V, 0, 1);
   const uint4* xv = reinterpret_cast<const uint4*>(x + slice.head);
   // stretches of whole vectors; the first warp has the elements in front of the vectors, too, the last those behind
   const int per = (slice.vectors + WARPS - 1) / WARPS, v0 = min(slice.vectors, warp * per), v1 = min(slice.vectors, v0 + per);
-  const int tail = slice.head + slice.vectors * N;
-  auto equals = [&](const uint4& u) {
-    const T* e = reinterpret_cast<const T*>(&u);
-    unsigned int m = 0u;
+  const int tail = slice.element(slice.vectors);
+  unsigned int n = 0u, kept[KEEP];   // the first eight rounds' places stay in registers (rows up to 65 536 bf16)
+  if (warp == 0 && lane < slice.head) n += to_float(x[lane]) == number;
+  if (warp == WARPS - 1 && tail + lane < V) n += to_float(x[tail + lane]) == number;
 #pragma unroll
-    for (int i = 0; i < N; ++i) m |= (VocabKey<T>::of(e[i]) == key ? 1u : 0u) << i;
-    return m;
-  };
-  unsigned int n = 0u;
-  if (warp == 0 && lane < slice.head) n += VocabKey<T>::of(x[lane]) == key;
-  if (warp == WARPS - 1 && tail + lane < V) n += VocabKey<T>::of(x[tail + lane]) == key;
-  for (int v = v0 + lane; v < v1; v += 32) n += __popc(equals(__ldg(xv + v)));
+  for (int i = 0; i < KEEP; ++i) {
+    const int v = v0 + 32 * i + lane;
+    kept[i] = v < v1 ? vs_equal<T>(__ldg(xv + v), value) : 0u;
+    n += __popc(kept[i]);
+  }
+  for (int v = v0 + 32 * KEEP + lane; v < v1; v += 32) n += __popc(vs_equal<T>(__ldg(xv + v), value));
   n = __reduce_add_sync(0xffffffffu, n);
   __syncthreads();
   if (lane == 0) wc[warp] = n;
   __syncthreads();
-  unsigned int before = 0u;
-  for (int w = 0; w < warp; ++w) before += wc[w];
+  unsigned int before = __reduce_add_sync(0xffffffffu, lane < warp ? wc[lane] : 0u);
   if (rank < before || rank >= before + n) return;
   auto single = [&](int j0, int j1) {
-    const bool hit = j0 + lane < j1 && VocabKey<T>::of(x[j0 + lane]) == key;
+    const bool hit = j0 + lane < j1 && to_float(x[j0 + lane]) == number;
     const unsigned int mask = __ballot_sync(0xffffffffu, hit);
     if (hit && before + __popc(mask & ((1u << lane) - 1u)) == rank) *out = j0 + lane;
     before += __popc(mask);
   };
-  if (warp == 0) single(0, slice.head);
-  for (int v = v0; v < v1; v += 32) {
-    const unsigned int m = v + lane < v1 ? equals(__ldg(xv + v + lane)) : 0u;
-    unsigned int upto = __popc(m);
+  auto round = [&](unsigned int m, int v) {
+    const unsigned int sum = __reduce_add_sync(0xffffffffu, __popc(m));
+    if (rank < before + sum && rank >= before) {   // here
+      unsigned int upto = __popc(m);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned int c = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += c;
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned int c = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += c;
+      }
+      unsigned int at = before + upto - __popc(m);
+      for (unsigned int b = m; b; b &= b - 1u, ++at)
+        if (at == rank) *out = slice.element(v + lane) + __ffs(b) - 1;
     }
-    unsigned int at = before + upto - __popc(m);
-    for (unsigned int b = m; b; b &= b - 1u, ++at)
-      if (at == rank) *out = slice.element(v + lane) + __ffs(b) - 1;
-    before += __shfl_sync(0xffffffffu, upto, 31);
-  }
+    before += sum;
+  };
+  if (warp == 0) single(0, slice.head);
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) round(kept[i], v0 + 32 * i);
+  for (int v = v0 + 32 * KEEP; v < v1; v += 32) round(v + lane < v1 ? vs_equal<T>(__ldg(xv + v + lane), value) : 0u, v);
   if (warp == WARPS - 1) single(tail, V);
 }
 
 // ---------------------------------------------------------------------------------------------- list
 // From the n entries in order (those that can be kept, all of them if fewer than top_k)
 template <typename T, int THREADS>
-__device__ void vs_listed_sample(VsScan<THREADS>& scan, const u64* list, const VsWeights<T>& w, const VsSettings& set, int n, int64_t* out) {
-  constexpr int PER = SEL_CAP / THREADS, SHIFT = 32 - VocabKey<T>::BITS;
+__device__ void vs_listed_sample(VsScan<THREADS>& scan, const u64* list, const VsWeights& w, const VsSettings& set, int n, int64_t* out) {
+  constexpr int PER = SEL_CAP / THREADS;
   const int tid = threadIdx.x;
   n = min(n, set.top_k);
   const int per = (n + THREADS - 1) / THREADS, i0 = min(n, tid * per);
@@ -437,8 +547,8 @@ __device__ void vs_listed_sample(VsScan<THREADS>& scan, const u64* list, const V
   for (int i = 0; i < PER; ++i) {
     each[i] = 0ull;
     if (i < per && i0 + i < n) {
-      const double v = w.of((uint32_t)(list[i0 + i] >> 32) >> SHIFT);
-      each[i] = VsWeights<T>::whole(v);
+      const double v = w.of(list_value<T>(list[i0 + i]));
+      each[i] = VsWeights::whole(v);
       if (v >= (double)set.min_p) over += each[i];
       mass += each[i];
     }
@@ -508,61 +618,77 @@ template <typename T, int THREADS> constexpr size_t vs_smem() {
   return vs_counting<T, THREADS>() && sizeof(VsCounts) > sizeof(VsDigits<THREADS>) ? sizeof(VsCounts) : sizeof(VsDigits<THREADS>);
 }
 
-template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) sample_kernel(const xl_sample_params p, const int blocks) {
+template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) sample_kernel(const xl_sample_params p, const double icap, const int blocks) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ SelShared<THREADS> ss;
   __shared__ VsScan<THREADS> scan;
+  __shared__ double invT;   // a 64-bit division: by one thread, and out of the way early
   const int rank = blocks > 1 ? (int)cluster_ctarank() : 0;
   const long long row = blockIdx.x / blocks;
   const VsSettings set(p, row);
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
+  if (threadIdx.x == 0) invT = 1.0 / (double)set.temperature;   // (read behind the first barrier)
   if (!(set.temperature > 0.f)) {
     if (rank == 0) vs_greedy<T, THREADS>(x, p.V, p.cap, p.tokens + row);
     return;
   }
   const bool few = set.top_k <= VS_LIST_K || p.V <= SEL_CAP, alone = !few && set.top_k == p.V && set.top_p >= 1.f && set.min_p > 0.f;
-  Selector<T, THREADS> sel(ss, x, p.V, rank, blocks);
-  sel.bound(few ? set.top_k : 1);
-  const float largest = float_of_key(ss.top);
-  if (!(largest > -INFINITY)) {
-    if (rank == 0 && threadIdx.x == 0) p.tokens[row] = 0;
-    return;
-  }
-  VsWeights<T> w;
-  w.set(p.cap, set.temperature, largest);
-  if (few || alone) {
-    float least = sel.least();
-    if (alone) {   // the smallest key of weight min_p, five bits at a time: every lane asks for one of 32
-      uint32_t key = 0u;
-      for (int shift = VocabKey<T>::BITS; shift > 0;) {
-        const int step = shift < 5 ? shift : 5, lane = threadIdx.x & 31;
-        shift -= step;
-        const uint32_t mine = key | (uint32_t)lane << shift | ((1u << shift) - 1u);   // the largest key of the lane's stretch
-        const bool in = lane >> step == 0 && (mine >= w.kmax || w.of(mine) >= (double)set.min_p);
-        const unsigned int some = __ballot_sync(0xffffffffu, in);
-        key |= (uint32_t)(some ? __ffs(some) - 1 : 0) << shift;
-      }
-      least = fminf(VocabKey<T>::value(key), largest);
-    }
-    sel.collect(least, [](const uint4&, int) {}, [](T) {});
-    __syncthreads();
-    const unsigned int n = sel.gather();
-    if (rank != 0) return;
-    if (n <= SEL_CAP && (alone || n >= (unsigned int)set.top_k || ss.bound == 0u)) {
-      sort_list<THREADS>(ss.list, (int)n);
-      vs_listed_sample<T, THREADS>(scan, ss.list, w, set, (int)n, p.tokens + row);
-      return;
-    }
-  }
-  if (rank != 0) return;
+  VsWeights w;
+  auto weigh = [&](float largest) {
+    w.set(p.cap, icap, invT, largest);
+  };
   VsPlace place;
   bool found = false;
+  if (few || alone || !vs_counting<T, THREADS>()) {
+    Selector<T, THREADS> sel(ss, x, p.V, rank, blocks);
+    sel.bound(few ? set.top_k : 1);
+    const float largest = float_of_key(ss.top);
+    if (!(largest > -INFINITY)) {
+      if (rank == 0 && threadIdx.x == 0) p.tokens[row] = 0;
+      return;
+    }
+    weigh(largest);
+    if (few || alone) {
+      float least = sel.least();
+      if (alone) {   // the smallest key of weight min_p, five bits at a time: every lane asks for one of 32
+        uint32_t key = 0u;
+        const uint32_t kmax = VocabKey<T>::of(from_float<T>(largest));
+        for (int shift = VocabKey<T>::BITS; shift > 0;) {
+          const int step = shift < 5 ? shift : 5, lane = threadIdx.x & 31;
+          shift -= step;
+          const uint32_t mine = key | (uint32_t)lane << shift | ((1u << shift) - 1u);   // the largest key of the lane's stretch
+          const bool in = lane >> step == 0 && (mine >= kmax || w.of(VocabKey<T>::value(mine)) >= (double)set.min_p);
+          const unsigned int some = __ballot_sync(0xffffffffu, in);
+          key |= (uint32_t)(some ? __ffs(some) - 1 : 0) << shift;
+        }
+        least = fminf(VocabKey<T>::value(key), largest);
+      }
+      sel.collect(least, [](const uint4&, int) {}, [](T) {});
+      __syncthreads();
+      const unsigned int n = sel.gather();
+      if (rank != 0) return;
+      if (n <= SEL_CAP && (alone || n >= (unsigned int)set.top_k || ss.bound == 0u)) {
+        sort_list<THREADS>(ss.list, (int)n);
+        vs_listed_sample<T, THREADS>(scan, ss.list, w, set, (int)n, p.tokens + row);
+        return;
+      }
+    }
+  }
   if constexpr (vs_counting<T, THREADS>()) {
     VsCounts& s = *reinterpret_cast<VsCounts*>(smem);
-    int values;
-    if (vs_counts<THREADS>(s, scan, x, p.V, &values)) {
-      place = vs_counted_sample<THREADS>(s, scan, w, set, values, p.V);
+    if (vs_counts<THREADS>(s, x, p.V)) {
+      const float largest = s.values ? __bfloat162float(__ushort_as_bfloat16((unsigned short)(s.value[0] >> 16))) : -INFINITY;
+      if (!(largest > -INFINITY)) {
+        if (threadIdx.x == 0) p.tokens[row] = 0;
+        return;
+      }
+      weigh(largest);
+      place = vs_counted_sample<THREADS>(s, scan, w, set);
       found = true;
+    } else if (!few && !alone) {   // (the digits need the largest logit)
+      Selector<T, THREADS> sel(ss, x, p.V, 0, 1);
+      sel.bound(1);
+      weigh(float_of_key(ss.top));
     }
     __syncthreads();
   }
@@ -589,7 +715,7 @@ template <typename T, int THREADS> static int vs_go(const xl_sample_params* p, i
   attr[0].val.clusterDim = {(unsigned)blocks, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, *p, blocks));
+  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, *p, p->cap > 0.f ? 1.0 / (double)p->cap : 0.0, blocks));
   return check_launch("xl_softcap_sample");
 }
 

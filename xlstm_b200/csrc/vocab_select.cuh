@@ -1,10 +1,10 @@
 // The largest logits of a row, sorted, without sorting the row.
 //
-// Mathematics.  Every thread keeps the largest logit of two groups of the row (the even and the odd places of its vectors).
-// If the k-th largest of the group maxima is t, at least k logits are >= t: t bounds the k-th largest logit from below, and with
-// G groups and k well below G only about -G ln(1 - k/G) logits reach it (71 for k = 64, G = 512).  So a first pass takes maxima, one
-// warp finds t by bisection over the leading 16 bits of the keys, a second pass collects what reaches t into a list, and only
-// the list is sorted, by (key, lower index).  Rows where too many logits reach t (crowds of equal ones, or all large logits in few
+// Mathematics.  The row falls into G groups of places (a thread's vectors, or the even and the odd places of them apart).  If the
+// k-th largest of the group maxima is t, at least k logits are >= t: t bounds the k-th largest logit from below, and only about
+// -G ln(1 - k/G) logits reach it (74 for k = 64, G = 256).  So a first pass takes maxima, one warp finds t by bisection over the
+// leading 16 bits of the keys -- its 16 rounds over G keys are a chain that the whole block waits for, hence no more groups
+// than k needs --, a second pass collects what reaches t into a list, and only the list is sorted, by (key, lower index).  Rows where too many logits reach t (crowds of equal ones, or all large logits in few
 // groups) are told by the length of the list, and left to the caller's exact selection.
 //
 // A row may be cut over a cluster of blocks: each finds the bound of its slice, the largest of the bounds holds for the row, and
@@ -17,6 +17,7 @@ namespace xl {
 
 constexpr int SEL_CAP = 1024;      // entries of the list
 constexpr int SEL_BLOCKS = 8;
+constexpr int SEL_GROUPS = 512, SEL_FEW = 96;   // groups; half of them up to this k
 constexpr int SEL_RANKED = 256;    // lists up to this length are sorted by counting who is larger
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
@@ -33,7 +34,7 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm 
 
 template <int THREADS> struct SelShared {
   unsigned long long list[SEL_CAP];     // key (32 bits) and ~index
-  unsigned short group[2 * THREADS];    // leading 16 bits of the groups' largest keys
+  unsigned short group[SEL_GROUPS];     // leading 16 bits of the groups' largest keys
   unsigned int from[2][SEL_BLOCKS];     // of the row's blocks: bound, largest key; written once a launch
   unsigned int largest[THREADS / 32];
   unsigned int n;                       // entries that reached the bound, also those beyond the list
@@ -104,27 +105,31 @@ template <typename T, int THREADS> struct Selector {
     GroupMax<T> g;
     for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int) { g.add(u); });
     for (int i = tid; i < singles; i += THREADS) g.add_one(x[slice.single(i, rank)]);
-    s.group[2 * tid] = (unsigned short)(key_of_float(g.even()) >> 16);
-    s.group[2 * tid + 1] = (unsigned short)(key_of_float(g.odd()) >> 16);
+    // 512 groups, or 256
+    const bool half = k <= SEL_FEW;
+    uint32_t ge = key_of_float(g.even()) >> 16, go = key_of_float(g.odd()) >> 16;
+#pragma unroll
+    for (int o = 1; o < 2 * THREADS / SEL_GROUPS; o <<= 1) {   // (of several threads together)
+      ge = max(ge, __shfl_xor_sync(0xffffffffu, ge, o));
+      go = max(go, __shfl_xor_sync(0xffffffffu, go, o));
+    }
+    constexpr int SHARE = 2 * THREADS / SEL_GROUPS;
+    if (tid % SHARE == 0 && k > 1) {
+      if (half) {
+        s.group[tid / SHARE] = (unsigned short)max(ge, go);
+      } else {
+        s.group[2 * (tid / SHARE)] = (unsigned short)ge;
+        s.group[2 * (tid / SHARE) + 1] = (unsigned short)go;
+      }
+    }
     const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of_float(fmaxf(g.even(), g.odd())));
     if (lane == 0) s.largest[tid >> 5] = mine;
     if (tid == 0) s.n = 0u;
     __syncthreads();
     if (tid < 32) {
-      constexpr int PER = 2 * THREADS / 64;   // pairs a lane
       const uint32_t* two = reinterpret_cast<const uint32_t*>(s.group);
-      uint32_t key[PER];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) key[i] = two[i * 32 + lane];
       const uint32_t top = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s.largest[lane] : 0u);
-      uint32_t t = 0u;
-      for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-        const uint32_t c = t | bit;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) n += (key[i] >> 16 >= c) + ((key[i] & 0xffffu) >= c);
-        if (__reduce_add_sync(0xffffffffu, n) >= k) t = c;
-      }
+      const uint32_t t = k == 1 ? top >> 16 : half ? bisect<SEL_GROUPS / 128>(two, k) : bisect<SEL_GROUPS / 64>(two, k);
       if (blocks > 1) {
         __syncwarp();
         cluster_wait();
@@ -149,6 +154,23 @@ template <typename T, int THREADS> struct Selector {
       }
     }
     __syncthreads();
+  }
+
+  // the k-th largest of 64 PAIRS keys (0 where there are fewer than k), by one warp
+  template <int PAIRS> static __device__ __forceinline__ uint32_t bisect(const uint32_t* two, int k) {
+    const int lane = threadIdx.x & 31;
+    uint32_t key[PAIRS], t = 0u;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) key[i] = two[i * 32 + lane];
+#pragma unroll 1
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+      const uint32_t c = t | bit;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) n += (key[i] >> 16 >= c) + ((key[i] & 0xffffu) >= c);
+      if (__reduce_add_sync(0xffffffffu, n) >= k) t = c;
+    }
+    return t;
   }
 
   // the bound as a number; -inf where there are too few groups for one
