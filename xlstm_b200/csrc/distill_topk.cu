@@ -12,7 +12,10 @@
 
 namespace xl {
 
-constexpr int DT_THREADS = 256, DT_WARPS = DT_THREADS / 32, DT_BLOCKS = 8;
+constexpr int DT_WARPS = 8, DT_BLOCKS = 8;   // warps: at most
+// threads of a block: small ones hide each other's serial parts best (2048 rows of 50 304: loss 59 us with 128, 63 with 256), but
+// with both directions in one launch the second pass finds more of its row in L1 where fewer rows are under way (265, 247 for 4096 rows)
+__host__ __device__ constexpr int dt_threads(bool both) { return both ? 256 : 128; }
 constexpr double DT_LN2 = 0.69314718055994530942;
 // what a row leaves for its gradient; the last two places hold a double
 enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_SMALL = 4, ST_REF = 5, ST_TEACHER = 6 };
@@ -76,11 +79,11 @@ template <int STEP, typename F> __device__ __forceinline__ void dt_vectors(const
 __device__ __forceinline__ double dt_nanmax(double a, double b) { return a != a || b != b ? a + b : fmax(a, b); }   // (NaN survives)
 
 template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD>
-__global__ void __launch_bounds__(DT_THREADS, 4) distill_kernel(const xl_distill_params p, const CappedZ<CAP> Z0, const double invT, const int blocks) {
+__global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8) distill_kernel(const xl_distill_params p, const CappedZ<CAP> Z0, const double invT, const int blocks) {
   CappedZ<CAP> Z = Z0;
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ DtShared s;
-  constexpr int N = Vec16<T>::N, THREADS = DT_THREADS, WARPS = DT_WARPS;
+  constexpr int N = Vec16<T>::N, THREADS = dt_threads(LOSS && GRAD), WARPS = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, K = p.K;
   const int rank = blocks > 1 ? (int)cluster_ctarank() : 0;
   const long long row = blockIdx.x / blocks;
@@ -419,22 +422,22 @@ static int dt_validate(const xl_distill_params* p) {
   return XL_OK;
 }
 
-// Blocks of a row.  One fills the machine from 592 rows on (four blocks an SM); fewer rows are cut into up to eight slices
+// Blocks of a row.  One fills the machine from 592 rows on (1024 threads an SM), or half that with small blocks; fewer rows are cut into up to eight slices
 // of at least 2048 tokens that exchange their sums through the cluster's shared memory.
-static int dt_blocks(int rows, int V) {
+static int dt_blocks(int rows, int V, bool both) {
   int blocks = 1;
-  while (blocks < DT_BLOCKS && rows * (blocks * 2) <= 4 * 148 && V >= 2048 * (blocks * 2)) blocks *= 2;
+  while (blocks < DT_BLOCKS && rows * (blocks * 2) <= (both ? 4 : 8) * 148 && V >= 2048 * (blocks * 2)) blocks *= 2;
   return blocks;
 }
 
 template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD> static int dt_go(const xl_distill_params* p, cudaStream_t st) {
-  const int blocks = dt_blocks(p->rows, p->V);
+  const int blocks = dt_blocks(p->rows, p->V, LOSS && GRAD);
   auto kern = distill_kernel<T, CAP, BOUNDED, LOSS, GRAD>;
   const size_t smem = dt_smem(p->K, p->V, Vec16<T>::N, blocks);
   if (smem > 40 * 1024) XL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p->rows * blocks);
-  cfg.blockDim = dim3(DT_THREADS);
+  cfg.blockDim = dim3(dt_threads(LOSS && GRAD));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];

@@ -618,7 +618,7 @@ template <typename T, int THREADS> constexpr size_t vs_smem() {
   return vs_counting<T, THREADS>() && sizeof(VsCounts) > sizeof(VsDigits<THREADS>) ? sizeof(VsCounts) : sizeof(VsDigits<THREADS>);
 }
 
-template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) sample_kernel(const xl_sample_params p, const double icap, const int blocks) {
+template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(THREADS) sample_kernel(const xl_sample_params p, const double icap, const int blocks) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ SelShared<THREADS> ss;
   __shared__ VsScan<THREADS> scan;
@@ -640,7 +640,7 @@ template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) sa
   VsPlace place;
   bool found = false;
   if (few || alone || !vs_counting<T, THREADS>()) {
-    Selector<T, THREADS> sel(ss, x, p.V, rank, blocks);
+    Selector<T, THREADS, KEEP> sel(ss, x, p.V, rank, blocks);
     sel.bound(few ? set.top_k : 1);
     const float largest = float_of_key(ss.top);
     if (!(largest > -INFINITY)) {
@@ -664,7 +664,6 @@ template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) sa
         least = fminf(VocabKey<T>::value(key), largest);
       }
       sel.collect(least, [](const uint4&, int) {}, [](T) {});
-      __syncthreads();
       const unsigned int n = sel.gather();
       if (rank != 0) return;
       if (n <= SEL_CAP && (alone || n >= (unsigned int)set.top_k || ss.bound == 0u)) {
@@ -686,7 +685,7 @@ template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) sa
       place = vs_counted_sample<THREADS>(s, scan, w, set);
       found = true;
     } else if (!few && !alone) {   // (the digits need the largest logit)
-      Selector<T, THREADS> sel(ss, x, p.V, 0, 1);
+      Selector<T, THREADS, 0> sel(ss, x, p.V, 0, 1);
       sel.bound(1);
       weigh(float_of_key(ss.top));
     }
@@ -701,8 +700,8 @@ template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) sa
 
 // Rows whose tokens are surely few take narrow blocks, several of them an SM, and where there are idle SMs a cluster of them;
 // all others one wide block each, whose shared memory holds the counts.
-template <typename T, int THREADS> static int vs_go(const xl_sample_params* p, int blocks, cudaStream_t st) {
-  auto kern = sample_kernel<T, THREADS>;
+template <typename T, int THREADS, int KEEP> static int vs_go(const xl_sample_params* p, int blocks, cudaStream_t st) {
+  auto kern = sample_kernel<T, THREADS, KEEP>;
   const size_t smem = vs_smem<T, THREADS>();
   XL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
@@ -721,10 +720,12 @@ template <typename T, int THREADS> static int vs_go(const xl_sample_params* p, i
 
 template <typename T> static int vs_launch(const xl_sample_params* p, cudaStream_t st) {
   const bool few = p->V <= SEL_CAP || (!p->top_k_rows && p->top_k > 0 && p->top_k <= VS_LIST_K);
-  if (!few) return vs_go<T, VS_WIDE>(p, 1, st);
+  if (!few) return vs_go<T, VS_WIDE, 0>(p, 1, st);
   int blocks = 1;
-  while (blocks < SEL_BLOCKS && p->rows * (blocks * 2) <= 2 * 148 && p->V >= 4096 * (blocks * 2) && p->top_k * blocks * 4 <= SEL_CAP) blocks *= 2;
-  return vs_go<T, VS_NARROW>(p, blocks, st);
+  while (blocks < SEL_BLOCKS && p->rows * (blocks * 2) <= 2 * 148 && p->V >= 2048 * (blocks * 2) && p->top_k * blocks * 4 <= SEL_CAP) blocks *= 2;
+  const int vectors = p->V / Vec16<T>::N;
+  if ((vectors + blocks - 1) / blocks <= 8 * VS_NARROW) return vs_go<T, VS_NARROW, 8>(p, blocks, st);
+  return vs_go<T, VS_NARROW, 0>(p, blocks, st);
 }
 
 }  // namespace xl

@@ -8,7 +8,7 @@
 // groups) are told by the length of the list, and left to the caller's exact selection.
 //
 // A row may be cut over a cluster of blocks: each finds the bound of its slice, the largest of the bounds holds for the row, and
-// block 0 gathers the lists through the cluster's shared memory.
+// all write to the list of block 0 through the cluster's shared memory.
 #pragma once
 
 #include "vocab_row.cuh"
@@ -20,24 +20,21 @@ constexpr int SEL_BLOCKS = 8;
 constexpr int SEL_GROUPS = 512, SEL_FEW = 96;   // groups; half of them up to this k
 constexpr int SEL_RANKED = 256;    // lists up to this length are sorted by counting who is larger
 
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ uint32_t add_cluster_u32(uint32_t addr, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
+  return old;
 }
-__device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
-  unsigned long long v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-  return v;
-}
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 
 template <int THREADS> struct SelShared {
+  static constexpr int GROUPS = 2 * THREADS < SEL_GROUPS ? 2 * THREADS : SEL_GROUPS;
   unsigned long long list[SEL_CAP];     // key (32 bits) and ~index
-  unsigned short group[SEL_GROUPS];     // leading 16 bits of the groups' largest keys
+  unsigned short group[GROUPS];         // leading 16 bits of the groups' largest keys
   unsigned int from[2][SEL_BLOCKS];     // of the row's blocks: bound, largest key; written once a launch
   unsigned int largest[THREADS / 32];
-  unsigned int n;                       // entries that reached the bound, also those beyond the list
+  unsigned int n, mine;                 // entries that reached the bound, also those beyond the list: of the row (block 0's), of the slice
   unsigned int bound, top;              // leading 16 bits of the bound's key; key of the largest logit
 };
 
@@ -69,6 +66,28 @@ template <> struct GroupMax<float> {
   __device__ __forceinline__ float odd() const { return b; }
 };
 
+// places of a vector's elements that are >= v, as bits
+template <typename T> __device__ __forceinline__ unsigned int vec_reach(const uint4& u, float v);
+template <> __device__ __forceinline__ unsigned int vec_reach<__nv_bfloat16>(const uint4& u, float v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 two = __float2bfloat162_rn(v);   // (a bf16 number, or -inf)
+  unsigned int m = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m |= (__hge2_mask(h[i], two) & 0x00020001u) << (2 * i);   // bits 2 i and 2 i + 17
+  return (m | m >> 16) & 0xffu;
+}
+template <> __device__ __forceinline__ unsigned int vec_reach<float>(const uint4& u, float v) {
+  return (__uint_as_float(u.x) >= v ? 1u : 0u) | (__uint_as_float(u.y) >= v ? 2u : 0u) | (__uint_as_float(u.z) >= v ? 4u : 0u) | (__uint_as_float(u.w) >= v ? 8u : 0u);
+}
+template <typename T> __device__ __forceinline__ T vec_element(const uint4& u, int i);   // (selects: the vector stays in registers)
+template <> __device__ __forceinline__ __nv_bfloat16 vec_element<__nv_bfloat16>(const uint4& u, int i) {
+  const uint32_t w = i < 4 ? (i < 2 ? u.x : u.y) : (i < 6 ? u.z : u.w);
+  return __ushort_as_bfloat16((unsigned short)(i & 1 ? w >> 16 : w & 0xffffu));
+}
+template <> __device__ __forceinline__ float vec_element<float>(const uint4& u, int i) {
+  return __uint_as_float(i < 2 ? (i == 0 ? u.x : u.y) : (i == 2 ? u.z : u.w));
+}
+
 // f(vector, its number) for v, v + STEP, .. below end, four loads under way at a time
 template <int STEP, typename F> __device__ __forceinline__ void for_vectors(const uint4* xv, int v, int end, F f) {
 #pragma unroll 1
@@ -83,13 +102,15 @@ template <int STEP, typename F> __device__ __forceinline__ void for_vectors(cons
   for (; v < end; v += STEP) f(__ldg(xv + v), v);
 }
 
-template <typename T, int THREADS> struct Selector {
-  static constexpr int N = Vec16<T>::N;
+// KEEP: the slice has at most KEEP vectors a thread, which stay in registers between the passes; 0: it is read twice
+template <typename T, int THREADS, int KEEP> struct Selector {
+  static constexpr int N = Vec16<T>::N, GROUPS = SelShared<THREADS>::GROUPS;
   SelShared<THREADS>& s;
   const T* x;
   RowSlice<T> slice;
   int rank, blocks, singles;
   const uint4* xv;
+  uint4 kept[KEEP ? KEEP : 1];
 
   __device__ __forceinline__ Selector(SelShared<THREADS>& s_, const T* x_, int V, int rank_, int blocks_)
       : s(s_), x(x_), slice(x_, V, rank_, blocks_), rank(rank_), blocks(blocks_) {
@@ -103,17 +124,26 @@ template <typename T, int THREADS> struct Selector {
     const int tid = threadIdx.x, lane = tid & 31;
     if (blocks > 1) cluster_arrive();
     GroupMax<T> g;
-    for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int) { g.add(u); });
+    if (KEEP) {
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (slice.v0 + tid + i * THREADS < slice.v1) kept[i] = __ldg(xv + slice.v0 + tid + i * THREADS);
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (slice.v0 + tid + i * THREADS < slice.v1) g.add(kept[i]);
+    } else {
+      for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int) { g.add(u); });
+    }
     for (int i = tid; i < singles; i += THREADS) g.add_one(x[slice.single(i, rank)]);
-    // 512 groups, or 256
-    const bool half = k <= SEL_FEW;
+    // all groups, or half of them
+    const bool half = k <= SEL_FEW && GROUPS == SEL_GROUPS;
     uint32_t ge = key_of_float(g.even()) >> 16, go = key_of_float(g.odd()) >> 16;
 #pragma unroll
-    for (int o = 1; o < 2 * THREADS / SEL_GROUPS; o <<= 1) {   // (of several threads together)
+    for (int o = 1; o < 2 * THREADS / GROUPS; o <<= 1) {   // (of several threads together)
       ge = max(ge, __shfl_xor_sync(0xffffffffu, ge, o));
       go = max(go, __shfl_xor_sync(0xffffffffu, go, o));
     }
-    constexpr int SHARE = 2 * THREADS / SEL_GROUPS;
+    constexpr int SHARE = 2 * THREADS / GROUPS;
     if (tid % SHARE == 0 && k > 1) {
       if (half) {
         s.group[tid / SHARE] = (unsigned short)max(ge, go);
@@ -124,12 +154,12 @@ template <typename T, int THREADS> struct Selector {
     }
     const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of_float(fmaxf(g.even(), g.odd())));
     if (lane == 0) s.largest[tid >> 5] = mine;
-    if (tid == 0) s.n = 0u;
+    if (tid == 0) s.n = s.mine = 0u;
     __syncthreads();
     if (tid < 32) {
       const uint32_t* two = reinterpret_cast<const uint32_t*>(s.group);
       const uint32_t top = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s.largest[lane] : 0u);
-      const uint32_t t = k == 1 ? top >> 16 : half ? bisect<SEL_GROUPS / 128>(two, k) : bisect<SEL_GROUPS / 64>(two, k);
+      const uint32_t t = k == 1 ? top >> 16 : half ? bisect<GROUPS / 128>(two, k) : bisect<GROUPS / 64>(two, k);
       if (blocks > 1) {
         __syncwarp();
         cluster_wait();
@@ -178,49 +208,55 @@ template <typename T, int THREADS> struct Selector {
     return s.bound == 0u ? -INFINITY : VocabKey<T>::value(s.bound << (VocabKey<T>::BITS - 16));
   }
 
-  // Second pass over the slice: what reaches `least` into the list; `also(vector, number)` and `also_one(element)` see everything.
+  // Second pass over the slice: what reaches `least` into block 0's list; `also(vector, number)` and `also_one(element)` see
+  // everything.
   template <typename F, typename G> __device__ void collect(float least, F also, G also_one) {
     const int tid = threadIdx.x;
+    const uint32_t n0 = mapa_u32(smem_u32(&s.n), 0), list0 = mapa_u32(smem_u32(s.list), 0);
     auto take = [&](T e, int j) {
-      if (to_float(e) >= least && *const_cast<volatile unsigned int*>(&s.n) <= SEL_CAP) {   // (a crowd need not be counted)
-        const unsigned int at = atomicAdd(&s.n, 1u);
-        if (at < SEL_CAP) s.list[at] = (unsigned long long)list_key(e) << 32 | (uint32_t)~j;
+      if (*const_cast<volatile unsigned int*>(&s.mine) > SEL_CAP) return;   // (a crowd need not be counted)
+      const unsigned long long entry = (unsigned long long)list_key(e) << 32 | (uint32_t)~j;
+      const unsigned int mine = atomicAdd(&s.mine, 1u);
+      if (blocks == 1) {
+        if (mine < SEL_CAP) s.list[mine] = entry;
+      } else {
+        const unsigned int at = add_cluster_u32(n0, 1u);
+        if (at < SEL_CAP) st_cluster_u64(list0 + 8 * at, entry);
       }
     };
-    for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) {
+    auto look = [&](const uint4& u, int v) {
       also(u, v);
-      GroupMax<T> g;
-      g.add(u);
-      if (fmaxf(g.even(), g.odd()) >= least) {
-        const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int i = 0; i < N; ++i) take(e[i], slice.element(v) + i);
+      for (unsigned int m = vec_reach<T>(u, least); m; m &= m - 1u) {
+        const int i = __ffs(m) - 1;
+        take(vec_element<T>(u, i), slice.element(v) + i);
       }
-    });
+    };
+    if (KEEP) {
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (slice.v0 + tid + i * THREADS < slice.v1) look(kept[i], slice.v0 + tid + i * THREADS);
+    } else {
+      for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, look);
+    }
     for (int i = tid; i < singles; i += THREADS) {
       const int j = slice.single(i, rank);
       also_one(x[j]);
-      take(x[j], j);
+      if (to_float(x[j]) >= least) take(x[j], j);
     }
   }
 
-  // Behind a barrier of the block (and of the cluster): all lists of the row in block 0's.  Returns the row's number of entries there
-  // (above SEL_CAP: too many).  Every block has to come here; the others are done then.
+  // Behind collect(), by all blocks; the others than block 0 are done then and may end.  Returns the number of entries in block 0's
+  // list (above SEL_CAP: too many).  A barrier for block 0.
   __device__ unsigned int gather() {
-    if (blocks == 1) return s.n;
-    cluster_sync_all();
-    unsigned int n = s.n;
-    if (rank == 0) {
-      for (int r = 1; r < blocks; ++r) {
-        const unsigned int more = ld_cluster_u32(mapa_u32(smem_u32(&s.n), r));
-        const uint32_t from = mapa_u32(smem_u32(s.list), r);
-        for (unsigned int i = threadIdx.x; i < min(more, (unsigned int)SEL_CAP) && n + i < SEL_CAP; i += THREADS) s.list[n + i] = ld_cluster_u64(from + 8 * i);
-        n += more;
-      }
+    if (blocks == 1) {
+      __syncthreads();
+      return s.mine;
     }
     __syncwarp();
-    cluster_sync_all();
-    return n;
+    cluster_arrive();
+    if (rank != 0) return 0u;
+    cluster_wait();
+    return s.n;
   }
 };
 

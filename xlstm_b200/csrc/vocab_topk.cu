@@ -7,21 +7,19 @@
 
 namespace xl {
 
-constexpr int TK_THREADS = 256, TK_WARPS = TK_THREADS / 32;
-
-struct TkShared {
-  SelShared<TK_THREADS> sel;
-  SelExact<TK_THREADS> exact;
-  float wf[TK_WARPS], from[SEL_BLOCKS];
+template <int THREADS> struct TkShared {
+  SelShared<THREADS> sel;
+  SelExact<THREADS> exact;
+  float wf[THREADS / 32], from[SEL_BLOCKS];
 };
 
-template <typename T, bool CAP> __global__ void __launch_bounds__(TK_THREADS, 4) topk_kernel(const xl_topk_params p, const CappedZ<CAP> Z0, const int blocks) {
-  __shared__ TkShared s;
+template <typename T, bool CAP, int THREADS, int KEEP> __global__ void __launch_bounds__(THREADS, KEEP ? 2 : 1024 / THREADS) topk_kernel(const xl_topk_params p, const CappedZ<CAP> Z0, const int blocks) {
+  __shared__ TkShared<THREADS> s;
   constexpr int N = Vec16<T>::N;
   const int tid = threadIdx.x, k = p.k, rank = blocks > 1 ? (int)cluster_ctarank() : 0;
   const long long row = blockIdx.x / blocks;
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
-  Selector<T, TK_THREADS> sel(s.sel, x, p.V, rank, blocks);
+  Selector<T, THREADS, KEEP> sel(s.sel, x, p.V, rank, blocks);
   sel.bound(k);
   const float least = sel.least(), largest = float_of_key(s.sel.top);
   CappedZ<CAP> Z = Z0;
@@ -50,7 +48,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TK_THREADS, 4)
   if (!Z.small(Vec16<T>::largest(mag))) {   // a logit near the cap: this thread's vectors again
     acc[0] = acc[1] = 0ull;
 #pragma unroll 1
-    for (int v = sel.slice.v0 + tid; v < sel.slice.v1; v += TK_THREADS) {
+    for (int v = sel.slice.v0 + tid; v < sel.slice.v1; v += THREADS) {
       Vec16<T> a;
       a.set(__ldg(sel.xv + v));
       f32x2 z[N / 2];
@@ -61,7 +59,7 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TK_THREADS, 4)
   {
     float a0, a1;
     f2_unpack(f2_add(acc[0], acc[1]), a0, a1);
-    sum = block_reduce<TK_WARPS>(sum + (a0 + a1), OpSum(), s.wf);   // (a barrier: the list is there, too)
+    sum = block_reduce<THREADS / 32>(sum + (a0 + a1), OpSum(), s.wf);   // (a barrier: the list is there, too)
   }
   if (blocks > 1 && tid == 0) st_cluster_f32(mapa_u32(smem_u32(&s.from[rank]), 0), sum);
   __syncwarp();
@@ -75,12 +73,12 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TK_THREADS, 4)
     p.lse[row] = isinf(largest) && !CAP ? largest : (float)((log2((double)sum) + (double)zmax) * 0.69314718055994530942 + (CAP ? 0.0 : (double)Z.ref / (double)p.temperature));
   }
   if (n > SEL_CAP || n < (unsigned int)k) {
-    select_exact<T, TK_THREADS>(s.exact, s.sel.list, x, p.V, k);
-    sort_list<TK_THREADS>(s.sel.list, k);
+    select_exact<T, THREADS>(s.exact, s.sel.list, x, p.V, k);
+    sort_list<THREADS>(s.sel.list, k);
   } else {
-    sort_list<TK_THREADS>(s.sel.list, (int)n);
+    sort_list<THREADS>(s.sel.list, (int)n);
   }
-  for (int i = tid; i < k; i += TK_THREADS) {
+  for (int i = tid; i < k; i += THREADS) {
     const unsigned long long e = s.sel.list[i];
     const float v = list_value<T>(e);
     p.values[row * k + i] = CAP ? p.cap * Z.tanh_of(v) : v;
@@ -88,27 +86,34 @@ template <typename T, bool CAP> __global__ void __launch_bounds__(TK_THREADS, 4)
   }
 }
 
-// Blocks of a row: one, and up to eight where there are idle SMs; the bound of a slice is weaker than the row's, and all lists have
-// to fit into one (about twice k a slice).
+// Blocks of a row: one, and up to eight where there are idle SMs.  The bound of a slice is weaker than the row's, so the lists of
+// k blocks are k times as long, and all have to fit into one (1.2 - 1.4 k entries each).
 static int tk_blocks(int rows, int V, int k) {
   int blocks = 1;
-  while (blocks < SEL_BLOCKS && rows * (blocks * 2) <= 4 * 148 && V >= 4096 * (blocks * 2) && k * blocks * 4 <= SEL_CAP) blocks *= 2;
+  while (blocks < SEL_BLOCKS && rows * (blocks * 2) <= 4 * 148 && V >= 2048 * (blocks * 2) && k * blocks * 4 <= SEL_CAP) blocks *= 2;
   return blocks;
 }
 
-template <typename T, bool CAP> static int tk_go(const xl_topk_params* p, cudaStream_t st) {
-  const int blocks = tk_blocks(p->rows, p->V, p->k);
+template <typename T, bool CAP, int THREADS, int KEEP> static int tk_go(const xl_topk_params* p, int blocks, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p->rows * blocks);
-  cfg.blockDim = dim3(TK_THREADS);
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {(unsigned)blocks, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, topk_kernel<T, CAP>, *p, CappedZ<CAP>(p->cap, p->temperature), blocks));
+  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, topk_kernel<T, CAP, THREADS, KEEP>, *p, CappedZ<CAP>(p->cap, p->temperature), blocks));
   return check_launch("xl_softcap_topk");
+}
+
+// Slices of up to eight vectors a thread stay in registers; longer ones are read twice, and then small blocks hide each other's
+// serial parts best, as long as their 256 groups are enough for k.
+template <typename T, bool CAP> static int tk_launch(const xl_topk_params* p, cudaStream_t st) {
+  const int blocks = tk_blocks(p->rows, p->V, p->k), vectors = p->V / Vec16<T>::N;
+  if ((vectors + blocks - 1) / blocks <= 8 * 256) return tk_go<T, CAP, 256, 8>(p, blocks, st);
+  return p->k <= SEL_FEW ? tk_go<T, CAP, 128, 0>(p, blocks, st) : tk_go<T, CAP, 256, 0>(p, blocks, st);
 }
 
 }  // namespace xl
@@ -121,6 +126,6 @@ extern "C" int xl_softcap_topk(const xl_topk_params* p, void* cuda_stream) {
   if (p->k <= 0 || p->k > p->V || !vocab_temperature(p->temperature)) return XL_ERR_BAD_SHAPE;
   if (p->k > TOPK_MAX) return XL_ERR_TOO_LARGE;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-  if (p->dtype == XL_F32) return p->cap > 0.f ? tk_go<float, true>(p, st) : tk_go<float, false>(p, st);
-  return p->cap > 0.f ? tk_go<__nv_bfloat16, true>(p, st) : tk_go<__nv_bfloat16, false>(p, st);
+  if (p->dtype == XL_F32) return p->cap > 0.f ? tk_launch<float, true>(p, st) : tk_launch<float, false>(p, st);
+  return p->cap > 0.f ? tk_launch<__nv_bfloat16, true>(p, st) : tk_launch<__nv_bfloat16, false>(p, st);
 }
