@@ -56,9 +56,6 @@ template <typename F> __device__ __forceinline__ float dt_exchange(float v, floa
   return v;
 }
 
-// Bound: with a cap |z| <= a, so that sums of 2^z need no maximum in front: 2^a * 2^18 and 2^-a stay normal numbers.
-constexpr float DT_BOUND = 100.f;
-
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
@@ -450,7 +447,7 @@ template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD> static int d
 }
 
 template <typename T> static int dt_launch(const xl_distill_params* p, bool loss, cudaStream_t st) {
-  const bool cap = p->cap > 0.f, bounded = cap && 1.45 * (double)p->cap <= DT_BOUND * (double)p->temperature;
+  const bool cap = p->cap > 0.f, bounded = vocab_bounded(p->cap, p->temperature);
   if (!loss) return cap ? dt_go<T, true, true, false, true>(p, st) : dt_go<T, false, false, false, true>(p, st);
   if (p->dlogits) {
     if (bounded) return dt_go<T, true, true, true, true>(p, st);

@@ -224,6 +224,8 @@ template <typename T> struct RowSlice {
   }
 };
 
+// With a cap |z| <= a = cap log2(e) / T: up to 100, sums of 2^z need no maximum in front (2^a * 2^18 and 2^-a are normal numbers).
+static inline bool vocab_bounded(float cap, float temperature) { return cap > 0.f && 1.45 * (double)cap <= 100.0 * (double)temperature; }
 // temperatures of the entries that compute in fp32
 static inline bool vocab_temperature(float t) { return t >= 1e-4f && t <= 1e6f; }
 // what row-wise entries over logits check in common

@@ -79,6 +79,15 @@ template <> __device__ __forceinline__ unsigned int vec_reach<__nv_bfloat16>(con
 template <> __device__ __forceinline__ unsigned int vec_reach<float>(const uint4& u, float v) {
   return (__uint_as_float(u.x) >= v ? 1u : 0u) | (__uint_as_float(u.y) >= v ? 2u : 0u) | (__uint_as_float(u.z) >= v ? 4u : 0u) | (__uint_as_float(u.w) >= v ? 8u : 0u);
 }
+// whether one is (or is NaN)
+template <typename T> __device__ __forceinline__ bool vec_any(const uint4& u, float v);
+template <> __device__ __forceinline__ bool vec_any<__nv_bfloat16>(const uint4& u, float v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  return !__hblt2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])), __float2bfloat162_rn(v));
+}
+template <> __device__ __forceinline__ bool vec_any<float>(const uint4& u, float v) {
+  return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w))) >= v;
+}
 template <typename T> __device__ __forceinline__ T vec_element(const uint4& u, int i);   // (selects: the vector stays in registers)
 template <> __device__ __forceinline__ __nv_bfloat16 vec_element<__nv_bfloat16>(const uint4& u, int i) {
   const uint32_t w = i < 4 ? (i < 2 ? u.x : u.y) : (i < 6 ? u.z : u.w);
@@ -88,18 +97,18 @@ template <> __device__ __forceinline__ float vec_element<float>(const uint4& u, 
   return __uint_as_float(i < 2 ? (i == 0 ? u.x : u.y) : (i == 2 ? u.z : u.w));
 }
 
-// f(vector, its number) for v, v + STEP, .. below end, four loads under way at a time
-template <int STEP, typename F> __device__ __forceinline__ void for_vectors(const uint4* xv, int v, int end, F f) {
+// f(vector, its number) for v, v + STEP, .. below end, BATCH loads under way at a time
+template <int STEP, int BATCH, typename F> __device__ __forceinline__ void for_vectors(const uint4* xv, int v, int end, F f) {
 #pragma unroll 1
-  for (; v + 3 * STEP < end; v += 4 * STEP) {
-    uint4 u[4];
+  for (; v < end; v += BATCH * STEP) {
+    uint4 u[BATCH];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = __ldg(xv + v + i * STEP);
+    for (int i = 0; i < BATCH; ++i)
+      if (v + i * STEP < end) u[i] = __ldg(xv + v + i * STEP);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f(u[i], v + i * STEP);
+    for (int i = 0; i < BATCH; ++i)
+      if (v + i * STEP < end) f(u[i], v + i * STEP);
   }
-#pragma unroll 1
-  for (; v < end; v += STEP) f(__ldg(xv + v), v);
 }
 
 // KEEP: the slice has at most KEEP vectors a thread, which stay in registers between the passes; 0: it is read twice
@@ -132,7 +141,7 @@ template <typename T, int THREADS, int KEEP> struct Selector {
       for (int i = 0; i < KEEP; ++i)
         if (slice.v0 + tid + i * THREADS < slice.v1) g.add(kept[i]);
     } else {
-      for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int) { g.add(u); });
+      for_vectors<THREADS, 8>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int) { g.add(u); });
     }
     for (int i = tid; i < singles; i += THREADS) g.add_one(x[slice.single(i, rank)]);
     // all groups, or half of them
@@ -226,6 +235,7 @@ template <typename T, int THREADS, int KEEP> struct Selector {
     };
     auto look = [&](const uint4& u, int v) {
       also(u, v);
+      if (!vec_any<T>(u, least)) return;
       for (unsigned int m = vec_reach<T>(u, least); m; m &= m - 1u) {
         const int i = __ffs(m) - 1;
         take(vec_element<T>(u, i), slice.element(v) + i);
@@ -236,7 +246,7 @@ template <typename T, int THREADS, int KEEP> struct Selector {
       for (int i = 0; i < KEEP; ++i)
         if (slice.v0 + tid + i * THREADS < slice.v1) look(kept[i], slice.v0 + tid + i * THREADS);
     } else {
-      for_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, look);
+      for_vectors<THREADS, 4>(xv, slice.v0 + tid, slice.v1, look);
     }
     for (int i = tid; i < singles; i += THREADS) {
       const int j = slice.single(i, rank);

@@ -13,7 +13,7 @@ template <int THREADS> struct TkShared {
   float wf[THREADS / 32], from[SEL_BLOCKS];
 };
 
-template <typename T, bool CAP, int THREADS, int KEEP> __global__ void __launch_bounds__(THREADS, KEEP ? 2 : 1024 / THREADS) topk_kernel(const xl_topk_params p, const CappedZ<CAP> Z0, const int blocks) {
+template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> __global__ void __launch_bounds__(THREADS, KEEP ? 2 : 1024 / THREADS) topk_kernel(const xl_topk_params p, const CappedZ<CAP> Z0, const int blocks) {
   __shared__ TkShared<THREADS> s;
   constexpr int N = Vec16<T>::N;
   const int tid = threadIdx.x, k = p.k, rank = blocks > 1 ? (int)cluster_ctarank() : 0;
@@ -24,7 +24,7 @@ template <typename T, bool CAP, int THREADS, int KEEP> __global__ void __launch_
   const float least = sel.least(), largest = float_of_key(s.sel.top);
   CappedZ<CAP> Z = Z0;
   Z.set_ref(largest);
-  const float zmax = CAP ? Z(largest) : 0.f;
+  const float zmax = CAP && !BOUNDED ? Z(largest) : 0.f;   // what z is taken relative to
   float sum = 0.f;
   f32x2 acc[2] = {0ull, 0ull};
   const f32x2 shift = f2_dup(-zmax);
@@ -33,7 +33,7 @@ template <typename T, bool CAP, int THREADS, int KEEP> __global__ void __launch_
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
       float z0, z1;
-      f2_unpack(f2_add(z[i], shift), z0, z1);
+      f2_unpack(CAP && !BOUNDED ? f2_add(z[i], shift) : z[i], z0, z1);
       acc[i & 1] = f2_add(acc[i & 1], f2_pack(exp2_approx(z0), exp2_approx(z1)));
     }
   };
@@ -94,7 +94,7 @@ static int tk_blocks(int rows, int V, int k) {
   return blocks;
 }
 
-template <typename T, bool CAP, int THREADS, int KEEP> static int tk_go(const xl_topk_params* p, int blocks, cudaStream_t st) {
+template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> static int tk_go(const xl_topk_params* p, int blocks, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p->rows * blocks);
   cfg.blockDim = dim3(THREADS);
@@ -104,16 +104,20 @@ template <typename T, bool CAP, int THREADS, int KEEP> static int tk_go(const xl
   attr[0].val.clusterDim = {(unsigned)blocks, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, topk_kernel<T, CAP, THREADS, KEEP>, *p, CappedZ<CAP>(p->cap, p->temperature), blocks));
+  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, topk_kernel<T, CAP, BOUNDED, THREADS, KEEP>, *p, CappedZ<CAP>(p->cap, p->temperature), blocks));
   return check_launch("xl_softcap_topk");
 }
 
-// Slices of up to eight vectors a thread stay in registers; longer ones are read twice, and then small blocks hide each other's
-// serial parts best, as long as their 256 groups are enough for k.
-template <typename T, bool CAP> static int tk_launch(const xl_topk_params* p, cudaStream_t st) {
+// Slices of up to eight vectors a thread stay in registers; longer ones are read twice, by blocks of 256 threads, four an SM: with
+// eight of 128 so many rows are under way that L2 loses half of them before the second pass (4096 rows of 50 304: 173 us, 158).
+template <typename T, bool CAP, bool BOUNDED> static int tk_launch(const xl_topk_params* p, cudaStream_t st) {
   const int blocks = tk_blocks(p->rows, p->V, p->k), vectors = p->V / Vec16<T>::N;
-  if ((vectors + blocks - 1) / blocks <= 8 * 256) return tk_go<T, CAP, 256, 8>(p, blocks, st);
-  return p->k <= SEL_FEW ? tk_go<T, CAP, 128, 0>(p, blocks, st) : tk_go<T, CAP, 256, 0>(p, blocks, st);
+  if ((vectors + blocks - 1) / blocks <= 8 * 256) return tk_go<T, CAP, BOUNDED, 256, 8>(p, blocks, st);
+  return tk_go<T, CAP, BOUNDED, 256, 0>(p, blocks, st);
+}
+template <typename T> static int tk_choose(const xl_topk_params* p, cudaStream_t st) {
+  if (!(p->cap > 0.f)) return tk_launch<T, false, false>(p, st);
+  return vocab_bounded(p->cap, p->temperature) ? tk_launch<T, true, true>(p, st) : tk_launch<T, true, false>(p, st);
 }
 
 }  // namespace xl
@@ -126,6 +130,5 @@ extern "C" int xl_softcap_topk(const xl_topk_params* p, void* cuda_stream) {
   if (p->k <= 0 || p->k > p->V || !vocab_temperature(p->temperature)) return XL_ERR_BAD_SHAPE;
   if (p->k > TOPK_MAX) return XL_ERR_TOO_LARGE;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-  if (p->dtype == XL_F32) return p->cap > 0.f ? tk_launch<float, true>(p, st) : tk_launch<float, false>(p, st);
-  return p->cap > 0.f ? tk_launch<__nv_bfloat16, true>(p, st) : tk_launch<__nv_bfloat16, false>(p, st);
+  return p->dtype == XL_F32 ? tk_choose<float>(p, st) : tk_choose<__nv_bfloat16>(p, st);
 }
