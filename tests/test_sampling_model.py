@@ -1,0 +1,163 @@
+"""Sampling and top logits through the model mirror: generate, the continuous-batch decoder, a teacher's top logits, and a
+distillation step over them.  CPU: with the oracle as the cell (host logic).  GPU: the kernels."""
+import types
+
+import pytest
+import torch
+
+from oracle import vocab as V
+from test_large_model import _continuous_case, _oracle_cell
+from xlstm_b200.large_model import ContinuousDecoder, LargeConfig, LargeModel, Sampling, procedural_state_dict
+
+CFG = LargeConfig(embedding_dim=128, num_heads=2, num_blocks=2, vocab_size=64)
+SETTINGS = [Sampling(0.8, 20, 0.9, 0.0), Sampling(), Sampling(0.0), Sampling(1.2, 0, 1.0, 0.05), Sampling(1.0, 5), Sampling(0.7, 0, 0.8), Sampling(1.5, 1)]
+
+
+def _model(device):
+    kw = dict(cell_ops=_oracle_cell()) if device == "cpu" else {}
+    return LargeModel(CFG, procedural_state_dict(CFG, 4), device, torch.float32, **kw)
+
+
+def _alone(model, prompt, count, settings, numbers):
+    """Token by token with given numbers."""
+    last, state, out = prompt[None].to(model.device), None, []
+    for u in numbers.reshape(count, 1):
+        last, state = model.forward(last, state, sampling=settings, u=u)
+        out.append(last[0, 0])
+    return torch.stack(out).cpu()
+
+
+def test_generate_draws_what_the_oracle_draws_on_cpu():
+    model = _model("cpu")
+    prompt = torch.randint(0, 64, (3, 17), generator=torch.Generator().manual_seed(1))
+    s = Sampling(torch.tensor([0.9, 1.3, 0.0]), 12, 0.95, torch.tensor([0.0, 0.02, 0.0]))
+    a, _ = model.generate(prompt, 6, sampling=s, generator=torch.Generator().manual_seed(5))
+    b, _ = model.generate(prompt, 6, sampling=s, generator=torch.Generator().manual_seed(5))
+    assert torch.equal(a, b)
+    u = torch.rand(18, generator=torch.Generator().manual_seed(5)).reshape(6, 3)
+    greedy, _ = model.generate(prompt, 6)
+    assert torch.equal(a[2], greedy[2])                       # temperature 0
+    last, state = prompt, None
+    for i in range(6):
+        logits, state = model.forward(last, state, last_only=True)
+        raw = CFG.output_logit_soft_cap * torch.atanh(logits[:, -1].double() / CFG.output_logit_soft_cap)   # (fp32 logits: ties aside)
+        for r in range(2):
+            token, margin = V.sample_row(raw[r], CFG.output_logit_soft_cap, u[i, r], float(s.temperature[r]), 12, 0.95, float(s.min_p[r]))
+            assert token == int(a[r, i]) or margin < 1e-5
+        last = a[:, i:i + 1]
+
+
+def test_decoder_draws_the_same_tokens_in_any_company_on_cpu():
+    model = _model("cpu")
+    prompts, counts = _continuous_case()
+    runs = [ContinuousDecoder(model, 3, sampling=True).run(prompts, counts, sampling=SETTINGS, generator=torch.Generator().manual_seed(9)),
+            ContinuousDecoder(model, 2, sampling=True).run(prompts, counts, quantum=2, sampling=SETTINGS, generator=torch.Generator().manual_seed(9)),
+            ContinuousDecoder(model, 3, row_len=96, packed_admission=True, sampling=True).run(prompts, counts, sampling=SETTINGS,
+                                                                                             generator=torch.Generator().manual_seed(9))]
+    numbers = torch.rand(sum(counts), generator=torch.Generator().manual_seed(9)).split(counts)
+    for d, (p, c) in enumerate(zip(prompts, counts)):
+        want = _alone(model, p, c, SETTINGS[d], numbers[d])
+        assert all(torch.equal(r[d], want) for r in runs), d
+    for bad in (dict(sampling=SETTINGS[:3]), dict(sampling=Sampling(-1.0)), dict(sampling=Sampling(1.0, 0, 1.5)), dict(sampling=Sampling(torch.ones(3))), {}):
+        with pytest.raises(ValueError):
+            ContinuousDecoder(model, 3, sampling=True).run(prompts, counts, **bad)
+    with pytest.raises(ValueError):
+        ContinuousDecoder(model, 3).run(prompts, counts, sampling=Sampling())
+
+
+def test_top_logits_on_cpu():
+    model = _model("cpu")
+    tokens = torch.randint(0, 64, (2, 21), generator=torch.Generator().manual_seed(2))
+    values, ids, lse = model.top_logits(tokens, 7, 2.0)
+    logits, _ = model.forward(tokens)
+    assert values.shape == ids.shape == (2, 21, 7) and lse.shape == (2, 21)
+    torch.testing.assert_close(values, logits.topk(7, dim=-1).values)
+    torch.testing.assert_close(values, logits.gather(-1, ids.long()))
+    torch.testing.assert_close(lse, torch.logsumexp(logits / 2.0, -1))
+
+
+@pytest.mark.gpu
+def test_generate_with_a_captured_step_draws_the_eager_tokens():
+    model = _model("cuda")
+    prompt = torch.randint(0, 64, (3, 17), generator=torch.Generator().manual_seed(1)).cuda()
+    gen = lambda seed: torch.Generator(device="cuda").manual_seed(seed)   # noqa: E731
+    per_row = Sampling(torch.tensor([0.9, 1.3, 0.0]).cuda(), 12, 0.95, torch.tensor([0.0, 0.02, 0.0]).cuda())
+    for s in (Sampling(0.9, 10), Sampling(0.9, 10), Sampling(1.1, 0, 0.9), per_row, None, per_row):
+        eager, _ = model.generate(prompt, 8, sampling=s, generator=gen(5))
+        graphed, _ = model.generate(prompt, 8, use_cuda_graph=True, sampling=s, generator=gen(5))
+        assert torch.equal(eager, graphed)
+    other, _ = model.generate(prompt, 8, sampling=Sampling(2.0), generator=gen(6))
+    assert not torch.equal(other, model.generate(prompt, 8)[0])
+    model.release_graph()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [True, False])
+def test_decoder_draws_the_same_tokens_in_any_company_on_gpu(packed):
+    import xlstm_b200
+    model = _model("cuda")
+    prompts, counts = _continuous_case()
+    gen = lambda: torch.Generator(device="cuda").manual_seed(9)   # noqa: E731
+    dec = ContinuousDecoder(model, 3, packed_admission=packed, sampling=True)
+    assert dec.graphed
+    outs = dec.run(prompts, counts, sampling=SETTINGS, generator=gen())
+    sliced = dec.run(prompts, counts, quantum=3, park_on_host=True, sampling=SETTINGS, generator=gen())
+    assert dec.evictions > 0
+    one = dec.run(prompts, counts, sampling=Sampling(0.0))
+    xlstm_b200.check_device_status()
+    model.release_graph()
+    numbers = torch.rand(sum(counts), device="cuda", generator=gen()).split(counts)
+    for d, (p, c) in enumerate(zip(prompts, counts)):
+        want = _alone(model, p, c, SETTINGS[d], numbers[d])
+        assert torch.equal(outs[d], want) and torch.equal(sliced[d], want)
+        assert torch.equal(one[d], model.generate(p[None].cuda(), c)[0][0].cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_teacher_and_a_student_and_its_tokens(dtype):
+    """The operators as they are used together: a teacher's top logits of a packed batch, a student (sLSTM cell and head) that
+    is distilled from them -- in pieces with known weights, and through autograd --, and tokens drawn from its logits."""
+    import xlstm_b200
+    from xlstm_b200 import ops
+    teacher = LargeModel(CFG, procedural_state_dict(CFG, 4), "cuda", dtype)
+    g = torch.Generator().manual_seed(3)
+    B, S, NH, DH, T = 2, 48, 2, 64, 2.0
+    tokens = torch.randint(0, 64, (B, S), generator=g).cuda()
+    values, ids, lse = teacher.top_logits(tokens, 8, T, cu_seqlens=[0, 20, 48, 96])
+    alone = teacher.top_logits(tokens[1:], 8, T)
+    assert torch.equal(ids[1:], alone[1]) or dtype is torch.bfloat16
+    ids[0, 40:] = -1                                         # padding behind the first row's documents
+    weight = torch.full((B, S), 1.0 / (B * S)).cuda()
+    wx = (0.5 * torch.randn(B, S, 4 * NH * DH, generator=g)).bfloat16().cuda()
+    R = (0.05 * torch.randn(NH, DH, 4, DH, generator=g)).bfloat16().cuda()
+    bias = (0.1 * torch.randn(NH, 4, DH, generator=g)).cuda()
+    head = (torch.randn(64, NH * DH, generator=g) / 8).to(dtype).cuda()
+
+    def student(leaves):
+        h, _ = ops.SlstmFunction.apply(leaves[0], leaves[1], bias, None)
+        return h.transpose(1, 2).reshape(B, S, NH * DH).to(dtype) @ leaves[2].t()
+    grads = []
+    for way in ("autograd", "pieces", "plain"):
+        leaves = [t.clone().requires_grad_() for t in (wx, R, head)]
+        logits = student(leaves)
+        if way == "autograd":
+            (ops.distill_topk(logits, values, ids, 30.0, T, lse) * weight).sum().backward()
+        elif way == "pieces":
+            got = [ops.distill_topk_grad(logits[b].detach(), values[b], ids[b], weight[b], 30.0, T, lse[b])[1] for b in range(B)]
+            logits.backward(torch.stack(got))
+        else:
+            d = V.distill_grad(logits.detach().double().cpu().reshape(B * S, 64), values.cpu().reshape(B * S, 8), ids.cpu().reshape(B * S, 8), 30.0, T,
+                               lse.cpu().reshape(B * S))
+            logits.backward((d.reshape(B, S, 64).cuda() * weight[..., None]).to(dtype))
+        grads.append([t.grad.double() for t in leaves])
+    xlstm_b200.check_device_status()
+    # the kernels' gradient of the logits is the formula's rounded once (fp32: a few 2^-24 more); what follows is the same code
+    tol = 2e-2 if dtype is torch.bfloat16 else 5e-3          # (bf16 roundings of dwx and R's gradient flip on last bits of dlogits: 2^-8 and a few)
+    for a, b, c in zip(*grads):
+        assert torch.isfinite(a).all()
+        assert float((a - c).norm() / c.norm()) < tol and float((b - c).norm() / c.norm()) < tol
+    assert torch.equal(grads[0][2] != 0, grads[2][2] != 0)
+    drawn = xlstm_b200.softcap_sample(logits.detach(), 30.0, torch.rand(B, S, generator=g).cuda(), 0.8, 10, 0.9)
+    kept = xlstm_b200.softcap_topk(logits.detach(), 30.0, 10)[1]
+    assert bool((kept == drawn[..., None]).any(-1).all())    # every token is one of its row's ten largest

@@ -57,6 +57,24 @@ class LargeConfig:
         return int(math.ceil(self.embedding_dim * self.ffn_proj_factor / m) * m)
 
 
+@dataclass
+class Sampling:
+    """How tokens are drawn from the capped logits (``ops.softcap_sample``): numbers for all rows, or tensors of one per row.
+    ``temperature`` 0 decodes greedily."""
+    temperature: object = 1.0
+    top_k: object = 0
+    top_p: object = 1.0
+    min_p: object = 0.0
+
+    def rows(self, index) -> "Sampling":
+        return Sampling(*(v[index] if torch.is_tensor(v) else v for v in (self.temperature, self.top_k, self.top_p, self.min_p)))
+
+    def key(self):
+        """What a captured step depends on; None where the settings lie in tensors (the step reads those anew)."""
+        vals = (self.temperature, self.top_k, self.top_p, self.min_p)
+        return None if any(torch.is_tensor(v) for v in vals) else vals
+
+
 def parameter_shapes(cfg: LargeConfig) -> dict:
     D, NH, F_, V = cfg.embedding_dim, cfg.num_heads, cfg.ffn_dim, cfg.vocab_size
     shapes = {"embedding.weight": (V, D), "backbone.out_norm.weight": (D,), "lm_head.weight": (V, D)}
@@ -100,6 +118,30 @@ def procedural_state_dict(cfg: LargeConfig, seed: int = 0, dtype=torch.float32, 
 
 def _soft_cap(x, cap):
     return cap * torch.tanh(x / cap)
+
+
+def _sample(logits, cap, u, s: Sampling):
+    """``ops.softcap_sample`` on any device, in 64-bit torch operations (the kernel is what runs on CUDA)."""
+    n = logits.shape[0]
+    T, k, p, mp = (torch.as_tensor(v, device=logits.device).expand(n)[:, None] for v in (s.temperature, s.top_k, s.top_p, s.min_p))
+    T, p, mp = T.float().double(), p.float().double(), mp.float().double()
+    x, idx = torch.sort(logits.double(), dim=-1, descending=True, stable=True)
+    y = _soft_cap(x, cap)
+    w = torch.exp((y - y[:, :1]) / T.clamp(min=1e-30))
+    w = torch.where((torch.arange(x.shape[1], device=x.device) < k) | (k <= 0), w, 0.0)
+    upto = torch.cumsum(w, -1)
+    keep = (((upto - w) < p * upto[:, -1:]) | (p >= 1)) & (w >= mp) & (w > 0)
+    keep[:, 0] = True
+    at = (upto <= u.double()[:, None] * torch.where(keep, w, 0.0).sum(-1, keepdim=True)).sum(-1)
+    drawn = idx.gather(1, torch.minimum(at, keep.sum(-1) - 1)[:, None])
+    return torch.where(T > 0, drawn, torch.argmax(_soft_cap(logits, cap), dim=-1, keepdim=True))
+
+
+def _top(logits, cap, k: int, temperature: float):
+    """``ops.softcap_topk`` on any device."""
+    y = _soft_cap(logits.float(), cap)
+    ids = torch.sort(logits, dim=-1, descending=True, stable=True).indices[..., :k]
+    return y.gather(-1, ids), ids.to(torch.int32), torch.logsumexp(y / temperature, -1)
 
 
 def _rms_norm(x, w, eps):
@@ -315,7 +357,7 @@ class LargeModel:
                 and (tokens.shape[0] * tokens.shape[1]) % self.tp_world == 0)
 
     def _forward_token_parallel(self, tokens, state, cu_seqlens, last_only, groups: int = 2, time_collectives: bool = False,
-                                greedy: bool = False):
+                                greedy: bool = False, sampling: Optional[Sampling] = None, u=None, top=None):
         """Prefill with the residual stream sharded over tokens (see the class docstring).  Batch rows are cut into
         `groups` independent pieces; piece g runs on stream g % 2, so its collectives overlap the other piece's compute."""
         cfg, W, dev = self.cfg, self.tp_world, self.device
@@ -353,10 +395,14 @@ class LargeModel:
                 xn_full = self._timed(self._gather_tokens, xn, record).reshape(Bg, S, -1)
                 if last_only:
                     xn_full = xn_full[:, -1:]
-                outs.append(self._head(xn_full, greedy))
+                rows = slice(g * Bg, (g + 1) * Bg)
+                outs.append(self._head(xn_full, greedy, None if sampling is None else sampling.rows(rows), None if u is None else u[rows], top))
         if cuda and len(streams) > 1:
             streams[0].wait_stream(streams[1])
-        logits = outs[0] if groups == 1 else torch.cat(outs, 0)
+        if top is not None:
+            logits = tuple(torch.cat(parts, 0) for parts in zip(*outs))
+        else:
+            logits = outs[0] if groups == 1 else torch.cat(outs, 0)
         new_state = {}
         for i in range(len(self.blocks)):
             parts = [pc["state"][i] for pc in pieces]
@@ -368,28 +414,45 @@ class LargeModel:
             self.comm_calls = len(record)
         return logits, new_state
 
-    def _head(self, xn, greedy: bool):
-        """lm_head and soft cap; with `greedy` the argmax of the last position as well (``generate.py:13-15``), on CUDA in
-        one kernel behind the GEMM."""
+    def _head(self, xn, greedy: bool, sampling: Optional[Sampling] = None, u=None, top=None):
+        """lm_head and soft cap; with `greedy` the argmax of the last position as well (``generate.py:13-15``), with `sampling` a
+        token drawn there by the numbers `u`, on CUDA in one kernel behind the GEMM.  `top` = (k, temperature): the k largest
+        logits of every position, their ids and the log-sum-exp, in pieces, so that the logits of all are never held at once."""
         cfg = self.cfg
+        cap = cfg.output_logit_soft_cap
+        if top is not None:
+            k, temperature = top
+            rows = xn.reshape(-1, xn.shape[-1])
+            parts = [ops.softcap_topk(piece, cap, k, temperature) if self.fused else _top(piece, cap, k, temperature)
+                     for piece in (self._linear(r, self.lm_head) for r in rows.split(4096))]
+            values, ids, lse = (torch.cat(p_) if len(parts) > 1 else p_[0] for p_ in zip(*parts))
+            lead = xn.shape[:-1]
+            return values.reshape(*lead, k), ids.reshape(*lead, k), lse.reshape(lead)
         logits = self._linear(xn, self.lm_head)
+        if sampling is not None:
+            rows = logits[:, -1]
+            if self.fused:
+                return ops.softcap_sample(rows, cap, u, sampling.temperature, sampling.top_k, sampling.top_p, sampling.min_p)[:, None]
+            return _sample(rows, cap, u, sampling)
         if greedy:
             if self.fused:
-                return ops.softcap_argmax(logits[:, -1], cfg.output_logit_soft_cap)[:, None]
-            return torch.argmax(_soft_cap(logits[:, -1:], cfg.output_logit_soft_cap), dim=-1)
-        return ops.soft_cap(logits, cfg.output_logit_soft_cap) if self.fused else _soft_cap(logits, cfg.output_logit_soft_cap)
+                return ops.softcap_argmax(logits[:, -1], cap)[:, None]
+            return torch.argmax(_soft_cap(logits[:, -1:], cap), dim=-1)
+        return ops.soft_cap(logits, cap) if self.fused else _soft_cap(logits, cap)
 
     def forward(self, tokens, state: Optional[dict] = None, cu_seqlens=None, slot=None, last_only: bool = False,
-                time_collectives: bool = False, positions=None, greedy: bool = False):
+                time_collectives: bool = False, positions=None, greedy: bool = False, sampling: Optional[Sampling] = None, u=None, top=None):
         """tokens (B,S) int64 -> logits (B,S,V) (or (B,1,V) with ``last_only``) and the per-block state dict
         ``{i: (c,n,m)}`` exactly as ``xLSTMLarge.forward`` returns it (``model.py:126-153``).  With ``cu_seqlens`` every
         interval of the flattened (B*S) token axis is a document of its own and the states have one row per document;
         ``positions`` (flat token indices) restricts the logits to those tokens, returned as (len(positions), 1, V) --
         a packed prefill only needs the last token of every document.  ``greedy`` returns the greedy token of the last
-        position, (rows, 1) int64, in place of the logits."""
+        position, (rows, 1) int64, in place of the logits; ``sampling`` a drawn one, by the uniform numbers ``u`` (rows,);
+        ``top`` = (k, temperature) what :meth:`top_logits` returns."""
+        greedy = greedy or sampling is not None
         if positions is None and self.token_parallel_ok(tokens, state, cu_seqlens, slot):
             return self._forward_token_parallel(tokens, state, cu_seqlens, last_only or greedy, time_collectives=time_collectives,
-                                                greedy=greedy)
+                                                greedy=greedy, sampling=sampling, u=u, top=top)
         cfg = self.cfg
         x = self.embedding[tokens]
         new_state = {}
@@ -410,11 +473,24 @@ class LargeModel:
         if pending is not None and not x.is_contiguous():
             x, pending = x.contiguous(), pending.contiguous()
         x, xn = self._reduce_add_norm(x, pending, self.out_norm)
-        return self._head(xn, greedy), new_state
+        return self._head(xn, greedy, sampling, u, top), new_state
 
     # ------------------------------------------------------------------------------------------------
-    def _capture_decode_graph(self, state, batch: int, slot_map=None):
-        """Capture one decode step (all blocks, lm_head, argmax) in a CUDA graph.  ``slot_map`` (int32, one entry per
+    @torch.no_grad()
+    def top_logits(self, tokens, k: int, temperature: float = 1.0, state=None, cu_seqlens=None):
+        """A teacher's view of `tokens` (B,S): ``values, ids, lse`` of :func:`ops.softcap_topk` for every position, (B,S,k),
+        (B,S,k) and (B,S) -- what ``ops.distill_topk`` takes.  The logits of more than 4096 positions are never held at once."""
+        return self.forward(tokens, state, cu_seqlens=cu_seqlens, top=(k, temperature))[0]
+
+    def _uniform(self, n: int, generator=None):
+        """n uniform numbers in [0, 1) on the model's device; with tensor parallelism the same on all ranks."""
+        u = torch.rand(n, device=self.device, generator=generator)
+        if self.tp_world > 1:
+            torch.distributed.broadcast(u, 0 if self.group is None else torch.distributed.get_global_rank(self.group, 0), group=self.group)
+        return u
+
+    def _capture_decode_graph(self, state, batch: int, slot_map=None, sampling: Optional[Sampling] = None):
+        """Capture one decode step (all blocks, lm_head, argmax or, with `sampling`, a draw by the numbers in ``_g_u``) in a CUDA graph.  ``slot_map`` (int32, one entry per
         row: the row's own index, or -1 while the row is free) makes the step kernel skip free rows, so an idle slot
         costs no state traffic.  The reference's decode loop
         (``generate.py:79-85``) launches every small operator from the host for every token; replaying a graph
@@ -427,9 +503,10 @@ class LargeModel:
         self._g_tok = torch.zeros(batch, 1, dtype=torch.long, device=dev)
 
         self._g_slot = slot_map
+        self._g_u = torch.zeros(batch, device=dev)
 
         def body():
-            nxt, st = self.forward(self._g_tok, self._g_state, greedy=True, slot=self._g_slot)
+            nxt, st = self.forward(self._g_tok, self._g_state, greedy=True, slot=self._g_slot, sampling=sampling, u=self._g_u)
             dsts, srcs = [], []
             for i, (c, n, m) in st.items():
                 assert c is self._g_state[i][0]
@@ -454,7 +531,7 @@ class LargeModel:
         for i, st in snapshot.items():   # undo the state changes of the warm-up and capture runs
             for dst, src in zip(self._g_state[i], st):
                 dst.copy_(src)
-        self._graph, self._graph_batch = graph, batch
+        self._graph, self._graph_batch, self._graph_sampling = graph, batch, sampling
 
     def parameters_on_device(self):
         """Every weight tensor this rank holds (its share under tensor parallelism)."""
@@ -468,38 +545,50 @@ class LargeModel:
         group is destroyed: a live graph that holds NCCL kernels keeps the communicator from shutting down."""
         self._graph = None
         self._g_state = None
-        self._g_tok = None
+        self._g_tok = self._g_u = self._graph_sampling = None
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
 
     @torch.no_grad()
-    def generate(self, prefill_tokens, max_length: int, state=None, use_cuda_graph: bool = False):
+    def generate(self, prefill_tokens, max_length: int, state=None, use_cuda_graph: bool = False, sampling: Optional[Sampling] = None,
+                 generator=None):
         """Greedy decoding as ``generate_tokens`` does it (``generate.py:79-85``): the first iteration consumes the
         prefill, every iteration appends argmax of the last position.  With ``use_cuda_graph`` the single-token
-        iterations replay a captured graph (same arithmetic, far fewer host launches)."""
-        out = torch.empty(prefill_tokens.shape[0], max_length, dtype=torch.long, device=self.device)
+        iterations replay a captured graph (same arithmetic, far fewer host launches).  With ``sampling`` every token is
+        drawn instead, by uniform numbers from ``generator`` (of the model's device; None: the default one)."""
+        B = prefill_tokens.shape[0]
+        out = torch.empty(B, max_length, dtype=torch.long, device=self.device)
+        u = None if sampling is None else self._uniform(max_length * B, generator).reshape(max_length, B)
         last = prefill_tokens
         for i in range(max_length):
             if use_cuda_graph and i >= 1:
                 if i == 1:
-                    B = prefill_tokens.shape[0]
-                    if getattr(self, "_graph", None) is None or self._graph_batch != B:
-                        self._capture_decode_graph(state, B)
+                    if getattr(self, "_graph", None) is None or self._graph_batch != B or not self._captured_for(sampling):
+                        self._capture_decode_graph(state, B, sampling=sampling)
                     else:   # load the fresh prefill state into the graph's static buffers
                         for j, st in state.items():
                             for dst, src in zip(self._g_state[j], st):
                                 dst.copy_(src.reshape(dst.shape))
                     self._g_tok.copy_(last)
+                if u is not None:
+                    self._g_u.copy_(u[i])
                 self._graph.replay()
                 out[:, i:i + 1] = self._g_tok
                 continue
-            last, state = self.forward(last, state, greedy=True)
+            last, state = self.forward(last, state, greedy=True, sampling=sampling, u=None if u is None else u[i])
             out[:, i:i + 1] = last
         if use_cuda_graph and max_length > 1:
             state = self._g_state
         if self.device.type == "cuda" and self.cell is ops:
             ops.check_device_status(self.device)   # synchronises; surfaces a kernel whose bounded wait expired
         return out, state
+
+    def _captured_for(self, sampling) -> bool:
+        """Whether the captured step draws its tokens as `sampling` says (settings in tensors: only for that very object)."""
+        had = self._graph_sampling
+        if had is None or sampling is None:
+            return had is sampling
+        return had is sampling or (had.key() is not None and had.key() == sampling.key())
 
 
 class ContinuousDecoder:
@@ -516,10 +605,15 @@ class ContinuousDecoder:
     documents' slots, their first tokens into the slots' token cells.  The reference's loop (``generate.py:27-90``) has no
     refill: it decodes one fixed batch to the end.  Token by token a stream computes what ``LargeModel.generate`` computes
     for it alone.  ``packed_admission=False`` prefills every document on its own (the CPU tests use it with the oracle
-    cell, which knows no document offsets)."""
+    cell, which knows no document offsets).
+
+    ``sampling=True`` makes a decoder whose slots draw their tokens: every slot has settings of its own (`run` takes them
+    per document; temperature 0 decodes greedily), which the captured step reads from vectors over the slots.  A document's
+    uniform numbers are drawn before the first step, one per token, so its tokens do not depend on its slot, its
+    company or on evictions beyond what the logits do."""
 
     def __init__(self, model: LargeModel, num_slots: int, use_cuda_graph: Optional[bool] = None, row_len: int = 32768,
-                 max_rows_per_prefill: int = 4, packed_admission: Optional[bool] = None):
+                 max_rows_per_prefill: int = 4, packed_admission: Optional[bool] = None, sampling: bool = False):
         from .sharding import SlotPool
         self.model, self.num_slots = model, num_slots
         cfg, dev = model.cfg, model.device
@@ -533,18 +627,28 @@ class ContinuousDecoder:
         self.slots = SlotPool(num_slots)
         self.slot_map = torch.full((num_slots,), -1, dtype=torch.int32, device=dev) if dev.type == "cuda" and model.cell is ops else None
         self.prefill_calls = 0
+        self.sampling = None
+        if sampling:
+            self.sampling = Sampling(torch.zeros(num_slots, device=dev), torch.zeros(num_slots, dtype=torch.int32, device=dev),
+                                     torch.ones(num_slots, device=dev), torch.zeros(num_slots, device=dev))
+            self.u = torch.zeros(num_slots, device=dev)
+            self.cursor = torch.zeros(num_slots, dtype=torch.long, device=dev)   # place of the slot's next number in `numbers`
+            self.numbers = torch.zeros(1, device=dev)
         if self.graphed:
             if self.slot_map is not None:
                 self.slot_map.copy_(torch.arange(num_slots, dtype=torch.int32, device=dev))   # capture with every row live
-            model._capture_decode_graph(self.state, num_slots, slot_map=self.slot_map)   # the graph's static buffers are this pool
+            model._capture_decode_graph(self.state, num_slots, slot_map=self.slot_map, sampling=self.sampling)   # the graph's static buffers are this pool
             self.state, self.tok = model._g_state, model._g_tok
+            if sampling:
+                self.u = model._g_u
             if self.slot_map is not None:
                 self.slot_map.fill_(-1)
 
     # ------------------------------------------------------------------------------------------------ admission
     @torch.no_grad()
     def _admit_single(self, slot: int, prompt: torch.Tensor) -> None:
-        first, st = self.model.forward(prompt.reshape(1, -1).to(self.model.device), greedy=True)
+        draw = self._drawing(torch.tensor([slot], dtype=torch.long, device=self.model.device))
+        first, st = self.model.forward(prompt.reshape(1, -1).to(self.model.device), greedy=True, **draw)
         self.prefill_calls += 1
         for i, (c, n, m) in st.items():
             self.state[i][0][slot].copy_(c[0])
@@ -577,10 +681,10 @@ class ContinuousDecoder:
                     continue
                 tokens[cu[k]:cu[k + 1]] = prompts[d].to(dev)
                 docs.append(d); rows_of_state.append(k); ends.append(cu[k + 1] - 1)
-            first, st = self.model.forward(tokens.reshape(r1 - r0, packed.row_len), cu_seqlens=cu, greedy=True,
-                                           positions=torch.tensor(ends, dtype=torch.long, device=dev))
-            self.prefill_calls += 1
             dst = torch.tensor([slots[d] for d in docs], dtype=torch.long, device=dev)
+            first, st = self.model.forward(tokens.reshape(r1 - r0, packed.row_len), cu_seqlens=cu, greedy=True,
+                                           positions=torch.tensor(ends, dtype=torch.long, device=dev), **self._drawing(dst))
+            self.prefill_calls += 1
             src = torch.tensor(rows_of_state, dtype=torch.long, device=dev)
             for i, (c, n, m) in st.items():
                 self.state[i][0].index_copy_(0, dst, c.index_select(0, src))
@@ -598,12 +702,36 @@ class ContinuousDecoder:
             idx = torch.tensor(slots, dtype=torch.long, device=self.model.device)
             self.slot_map.index_copy_(0, idx, idx.to(torch.int32))
 
+    # ------------------------------------------------------------------------------------------------ sampling
+    def _set_slot(self, slots, settings, cursors) -> None:
+        """The slots' settings and the places of their next uniform numbers."""
+        if self.sampling is None or not slots:
+            return
+        dev = self.model.device
+        at = torch.tensor(slots, dtype=torch.long, device=dev)
+        for field in ("temperature", "top_k", "top_p", "min_p"):
+            dst = getattr(self.sampling, field)
+            dst.index_copy_(0, at, torch.tensor([getattr(x, field) for x in settings], dtype=dst.dtype, device=dev))
+        self.cursor.index_copy_(0, at, torch.tensor(cursors, dtype=torch.long, device=dev))
+
+    def _drawing(self, at) -> dict:
+        """Arguments of a forward pass whose rows draw the next token of the slots `at`."""
+        if self.sampling is None:
+            return {}
+        u = self.numbers[self.cursor[at]]
+        self.cursor.index_add_(0, at, torch.ones_like(at))
+        return dict(sampling=self.sampling.rows(at), u=u)
+
     @torch.no_grad()
     def _step(self) -> None:
+        if self.sampling is not None:   # (a free slot's place may run past its document's numbers: any number will do)
+            torch.index_select(self.numbers, 0, self.cursor.clamp(max=self.numbers.numel() - 1), out=self.u)
+            self.cursor.add_(1)
         if self.graphed:
             self.model._graph.replay()
             return
-        nxt, st = self.model.forward(self.tok, self.state, greedy=True, slot=self.slot_map)
+        draw = {} if self.sampling is None else dict(sampling=self.sampling, u=self.u)
+        nxt, st = self.model.forward(self.tok, self.state, greedy=True, slot=self.slot_map, **draw)
         for i, (c, n, m) in st.items():
             for dst, src in zip(self.state[i], (c, n, m)):
                 if dst is not src:
@@ -633,19 +761,36 @@ class ContinuousDecoder:
             self.slot_map[slot] = slot
 
     @torch.no_grad()
-    def run(self, prompts, new_tokens, quantum: Optional[int] = None, park_on_host: bool = False):
+    def run(self, prompts, new_tokens, quantum: Optional[int] = None, park_on_host: bool = False, sampling=None, generator=None):
         """prompts: sequence of 1-D int64 tensors; new_tokens: int or per-document counts (>= 1).  Returns the list of
         generated token tensors in the order of ``prompts``.
 
         ``quantum``: with documents waiting and no slot free, a stream that has decoded ``quantum`` tokens since it was
         (re)admitted is EVICTED -- state and pending token parked (on the device, or on the host with ``park_on_host``) --
         and queues up behind the waiting documents; it later resumes from the parked state in whatever slot is free,
-        without a second prefill.  Tokens are the same with and without eviction."""
+        without a second prefill.  Tokens are the same with and without eviction.
+
+        ``sampling`` (of a decoder made with ``sampling=True``): one ``Sampling`` of numbers for all documents, or one each;
+        ``generator``: where the uniform numbers come from (of the model's device; None: the default one)."""
         counts = [int(new_tokens)] * len(prompts) if isinstance(new_tokens, int) else [int(x) for x in new_tokens]
         if len(counts) != len(prompts) or any(c < 1 for c in counts):
             raise ValueError("one positive token count per prompt")
         if quantum is not None and quantum < 1:
             raise ValueError("quantum must be positive")
+        if (sampling is not None) != (self.sampling is not None):
+            raise ValueError("settings for drawing tokens go with a decoder made with sampling=True")
+        start = [0] * len(counts)   # place of a document's first uniform number
+        if sampling is not None:
+            settings = [sampling] * len(counts) if isinstance(sampling, Sampling) else list(sampling)
+            if len(settings) != len(counts) or any(x.key() is None for x in settings):
+                raise ValueError("one Sampling of numbers per prompt")
+            for x in settings:
+                if not (x.temperature >= 0 and x.top_k >= 0 and 0 <= x.top_p <= 1 and 0 <= x.min_p <= 1):
+                    raise ValueError(f"sampling settings out of range: {x}")
+            for d in range(1, len(counts)):
+                start[d] = start[d - 1] + counts[d - 1]
+            if counts:
+                self.numbers = self.model._uniform(sum(counts), generator)
         queue = list(range(len(prompts)))[::-1]
         parked = {}          # document -> parcel of an evicted stream
         left = dict(enumerate(counts))   # document -> tokens still to produce
@@ -659,6 +804,9 @@ class ContinuousDecoder:
                 while queue and self.slots.free:
                     d = queue.pop()
                     (back if d in parked else fresh).append((self.slots.acquire(d), d))
+                if sampling is not None:
+                    self._set_slot([s_ for s_, _ in fresh + back], [settings[d] for _, d in fresh + back],
+                                   [start[d] + counts[d] - left[d] + (d in parked) for _, d in fresh + back])
                 if fresh:
                     self._admit([s_ for s_, _ in fresh], [prompts[d] for _, d in fresh])
                 for s_, d in back:
