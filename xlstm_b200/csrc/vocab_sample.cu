@@ -722,7 +722,7 @@ template <typename T> static int vs_launch(const xl_sample_params* p, cudaStream
   const bool few = p->V <= SEL_CAP || (!p->top_k_rows && p->top_k > 0 && p->top_k <= VS_LIST_K);
   if (!few) return vs_go<T, VS_WIDE, 0>(p, 1, st);
   int blocks = 1;
-  while (blocks < SEL_BLOCKS && p->rows * (blocks * 2) <= 2 * 148 && p->V >= 2048 * (blocks * 2) && p->top_k * blocks * 4 <= SEL_CAP) blocks *= 2;
+  while (blocks < SEL_BLOCKS && p->rows * (blocks * 2) <= 2 * 148 && p->V >= 2048 * (blocks * 2) && p->top_k * 3 <= SEL_CAP) blocks *= 2;
   const int vectors = p->V / Vec16<T>::N;
   if ((vectors + blocks - 1) / blocks <= 8 * VS_NARROW) return vs_go<T, VS_NARROW, 8>(p, blocks, st);
   return vs_go<T, VS_NARROW, 0>(p, blocks, st);

@@ -3,12 +3,12 @@
 // Mathematics.  The row falls into G groups of places (a thread's vectors, or the even and the odd places of them apart).  If the
 // k-th largest of the group maxima is t, at least k logits are >= t: t bounds the k-th largest logit from below, and only about
 // -G ln(1 - k/G) logits reach it (74 for k = 64, G = 256).  So a first pass takes maxima, one warp finds t by bisection over the
-// leading 16 bits of the keys -- its 16 rounds over G keys are a chain that the whole block waits for, hence no more groups
-// than k needs --, a second pass collects what reaches t into a list, and only the list is sorted, by (key, lower index).  Rows where too many logits reach t (crowds of equal ones, or all large logits in few
+// leading 16 bits of the keys -- the whole block waits for its rounds, hence no more groups than k needs --, a second pass
+// collects what reaches t into a list, and only the list is sorted, by (key, lower index).  Rows where too many logits reach t (crowds of equal ones, or all large logits in few
 // groups) are told by the length of the list, and left to the caller's exact selection.
 //
-// A row may be cut over a cluster of blocks: each finds the bound of its slice, the largest of the bounds holds for the row, and
-// all write to the list of block 0 through the cluster's shared memory.
+// A row may be cut over a cluster of b blocks: where every slice has k / b group maxima >= t the row has k, so the smallest of the
+// slices' (k / b)-th largest holds; all blocks write to the list of block 0 through the cluster's shared memory.
 #pragma once
 
 #include "vocab_row.cuh"
@@ -17,8 +17,7 @@ namespace xl {
 
 constexpr int SEL_CAP = 1024;      // entries of the list
 constexpr int SEL_BLOCKS = 8;
-constexpr int SEL_GROUPS = 512, SEL_FEW = 96;   // groups; half of them up to this k
-constexpr int SEL_RANKED = 256;    // lists up to this length are sorted by counting who is larger
+constexpr int SEL_GROUPS = 512;    // at most; as few of 64, 128, 256, 512 as 3/8 of them are k
 
 __device__ __forceinline__ uint32_t add_cluster_u32(uint32_t addr, uint32_t v) {
   uint32_t old;
@@ -111,6 +110,34 @@ template <int STEP, int BATCH, typename F> __device__ __forceinline__ void for_v
   }
 }
 
+// a warp's 32 values in descending order over its lanes
+template <typename V> __device__ __forceinline__ V run_sorted(V e) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int len = 2; len <= 32; len <<= 1)
+#pragma unroll
+    for (int step = len >> 1; step > 0; step >>= 1) {
+      const V o = __shfl_xor_sync(0xffffffffu, e, step);
+      const bool larger = ((lane & len) == 0) == ((lane & step) == 0);   // whether this lane keeps the larger one
+      e = (e > o) == larger ? e : o;
+    }
+  return e;
+}
+// how many values of the sorted runs but run `own` are larger than e
+template <typename V> __device__ __forceinline__ int above_in_runs(const V* list, int runs, int own, V e) {
+  int above = 0;
+#pragma unroll 4
+  for (int q = 0; q < runs; ++q) {
+    const V* run = list + 32 * q;
+    int c = 0;
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) c += run[c + step - 1] > e ? step : 0;
+    c += run[c] > e ? 1 : 0;   // (32 if all are larger)
+    above += q == own ? 0 : c;
+  }
+  return above;
+}
+
 // KEEP: the slice has at most KEEP vectors a thread, which stay in registers between the passes; 0: it is read twice
 template <typename T, int THREADS, int KEEP> struct Selector {
   static constexpr int N = Vec16<T>::N, GROUPS = SelShared<THREADS>::GROUPS;
@@ -144,22 +171,18 @@ template <typename T, int THREADS, int KEEP> struct Selector {
       for_vectors<THREADS, 8>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int) { g.add(u); });
     }
     for (int i = tid; i < singles; i += THREADS) g.add_one(x[slice.single(i, rank)]);
-    // all groups, or half of them
-    const bool half = k <= SEL_FEW && GROUPS == SEL_GROUPS;
+    // the groups' largest keys: of a thread's even and odd places, of both, of two or more threads together
+    k = (k + blocks - 1) / blocks;
+    int groups = 64;
+    while (groups < GROUPS && 8 * k > 3 * groups) groups *= 2;
     uint32_t ge = key_of_float(g.even()) >> 16, go = key_of_float(g.odd()) >> 16;
-#pragma unroll
-    for (int o = 1; o < 2 * THREADS / GROUPS; o <<= 1) {   // (of several threads together)
-      ge = max(ge, __shfl_xor_sync(0xffffffffu, ge, o));
-      go = max(go, __shfl_xor_sync(0xffffffffu, go, o));
-    }
-    constexpr int SHARE = 2 * THREADS / GROUPS;
-    if (tid % SHARE == 0 && k > 1) {
-      if (half) {
-        s.group[tid / SHARE] = (unsigned short)max(ge, go);
-      } else {
-        s.group[2 * (tid / SHARE)] = (unsigned short)ge;
-        s.group[2 * (tid / SHARE) + 1] = (unsigned short)go;
-      }
+    const bool both = groups < 2 * THREADS;
+    if (both) ge = max(ge, go);
+    const int share = both ? THREADS / groups : 1;   // threads of a group
+    for (int o = 1; o < share; o <<= 1) ge = max(ge, __shfl_xor_sync(0xffffffffu, ge, o));
+    if (k > 1 && tid % share == 0) {
+      s.group[tid / share] = (unsigned short)ge;
+      if (!both) s.group[THREADS + tid] = (unsigned short)go;
     }
     const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of_float(fmaxf(g.even(), g.odd())));
     if (lane == 0) s.largest[tid >> 5] = mine;
@@ -168,7 +191,9 @@ template <typename T, int THREADS, int KEEP> struct Selector {
     if (tid < 32) {
       const uint32_t* two = reinterpret_cast<const uint32_t*>(s.group);
       const uint32_t top = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s.largest[lane] : 0u);
-      const uint32_t t = k == 1 ? top >> 16 : half ? bisect<GROUPS / 128>(two, k) : bisect<GROUPS / 64>(two, k);
+      uint32_t t = top >> 16;
+      if (k > groups) t = 0u;
+      else if (k > 1) t = groups == 64 ? bisect<1>(two, k) : groups == 128 ? bisect<2>(two, k) : groups == 256 ? bisect<4>(two, k) : bisect<GROUPS / 64>(two, k);
       if (blocks > 1) {
         __syncwarp();
         cluster_wait();
@@ -186,8 +211,8 @@ template <typename T, int THREADS, int KEEP> struct Selector {
       __syncwarp();
       cluster_sync_all();
       if (tid == 0) {
-        uint32_t t = 0u, top = 0u;
-        for (int r = 0; r < blocks; ++r) { t = max(t, s.from[0][r]); top = max(top, s.from[1][r]); }
+        uint32_t t = 0xffffu, top = 0u;
+        for (int r = 0; r < blocks; ++r) { t = min(t, s.from[0][r]); top = max(top, s.from[1][r]); }
         s.bound = t;
         s.top = top;
       }
@@ -195,18 +220,27 @@ template <typename T, int THREADS, int KEEP> struct Selector {
     __syncthreads();
   }
 
-  // the k-th largest of 64 PAIRS keys (0 where there are fewer than k), by one warp
+  // the k-th largest of 64 PAIRS >= k keys, by one warp: bit by bit below the bits that all share
   template <int PAIRS> static __device__ __forceinline__ uint32_t bisect(const uint32_t* two, int k) {
     const int lane = threadIdx.x & 31;
-    uint32_t key[PAIRS], t = 0u;
+    uint32_t key[2 * PAIRS], lo = 0xffffu, hi = 0u;
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) key[i] = two[i * 32 + lane];
+    for (int i = 0; i < PAIRS; ++i) {
+      const uint32_t w = two[i * 32 + lane];
+      key[2 * i] = w >> 16;
+      key[2 * i + 1] = w & 0xffffu;
+      lo = min(lo, min(key[2 * i], key[2 * i + 1]));
+      hi = max(hi, max(key[2 * i], key[2 * i + 1]));
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    uint32_t bit = lo == hi ? 0u : 0x80000000u >> __clz(lo ^ hi), t = bit ? hi & ~(2u * bit - 1u) : hi;
 #pragma unroll 1
-    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+    for (; bit; bit >>= 1) {
       const uint32_t c = t | bit;
       int n = 0;
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) n += (key[i] >> 16 >= c) + ((key[i] & 0xffffu) >= c);
+      for (int i = 0; i < 2 * PAIRS; ++i) n += key[i] >= c;
       if (__reduce_add_sync(0xffffffffu, n) >= k) t = c;
     }
     return t;
@@ -222,10 +256,12 @@ template <typename T, int THREADS, int KEEP> struct Selector {
   template <typename F, typename G> __device__ void collect(float least, F also, G also_one) {
     const int tid = threadIdx.x;
     const uint32_t n0 = mapa_u32(smem_u32(&s.n), 0), list0 = mapa_u32(smem_u32(s.list), 0);
+    bool full = false;   // (a crowd need not be counted)
     auto take = [&](T e, int j) {
-      if (*const_cast<volatile unsigned int*>(&s.mine) > SEL_CAP) return;   // (a crowd need not be counted)
+      if (full) return;
       const unsigned long long entry = (unsigned long long)list_key(e) << 32 | (uint32_t)~j;
       const unsigned int mine = atomicAdd(&s.mine, 1u);
+      full = mine >= SEL_CAP;
       if (blocks == 1) {
         if (mine < SEL_CAP) s.list[mine] = entry;
       } else {
@@ -343,35 +379,35 @@ template <typename T, int THREADS> __device__ __noinline__ void select_exact(Sel
   __syncthreads();
 }
 
-// Descending sort of the n <= SEL_CAP entries (all different); ends behind a barrier.
+// Descending sort of the n <= SEL_CAP entries (all different, none zero); ends behind a barrier.  Every warp sorts runs of 32 in
+// registers; an entry's place then is its place in its run plus, from a binary search of each other run, how many are larger.
+// (223 entries: 4 900 cycles by comparing all with all, 352: 11 500 by a bitonic sort in shared memory.)
 template <int THREADS> __device__ void sort_list(unsigned long long* list, int n) {
-  const int tid = threadIdx.x;
-  if (n <= SEL_RANKED && n <= THREADS) {
-    const unsigned long long mine = tid < n ? list[tid] : 0ull;
-    int above = 0;
-    if ((tid & ~31) < n) {
-      int i = 0;
-      for (; i + 4 <= n; i += 4) above += (list[i] > mine) + (list[i + 1] > mine) + (list[i + 2] > mine) + (list[i + 3] > mine);
-      for (; i < n; ++i) above += list[i] > mine;
-    }
-    __syncthreads();
-    if (tid < n) list[above] = mine;
-    __syncthreads();
-    return;
+  constexpr int WARPS = THREADS / 32, PER = SEL_CAP / THREADS > 0 ? SEL_CAP / THREADS : 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, runs = (n + 31) / 32;
+  unsigned long long mine[PER];
+  int place[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = warp + i * WARPS, at = 32 * r + lane;
+    if (r >= runs) break;
+    mine[i] = run_sorted(at < n ? list[at] : 0ull);
+    list[at] = mine[i];   // (at < SEL_CAP: whole runs)
   }
-  int size = 1;
-  while (size < n) size <<= 1;
-  for (int i = n + tid; i < size; i += THREADS) list[i] = 0ull;
   __syncthreads();
-  for (int len = 2; len <= size; len <<= 1)
-    for (int step = len >> 1; step > 0; step >>= 1) {
-      for (int i = tid; i < size / 2; i += THREADS) {
-        const int a = 2 * i - (i & (step - 1)), b = a + step;
-        const unsigned long long u = list[a], v = list[b];
-        if ((u < v) == ((a & len) == 0)) { list[a] = v; list[b] = u; }
-      }
-      __syncthreads();
-    }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = warp + i * WARPS;
+    if (r >= runs) break;
+    place[i] = lane + above_in_runs<unsigned long long>(list, runs, r, mine[i]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (warp + i * WARPS >= runs) break;
+    if (mine[i]) list[place[i]] = mine[i];
+  }
+  __syncthreads();
 }
 
 }  // namespace xl

@@ -86,11 +86,11 @@ template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> __global__ 
   }
 }
 
-// Blocks of a row: one, and up to eight where there are idle SMs.  The bound of a slice is weaker than the row's, so the lists of
-// k blocks are k times as long, and all have to fit into one (1.2 - 1.4 k entries each).
+// Blocks of a row: one, and up to eight where there are idle SMs; the bound over slices is a little weaker, and the list should hold
+// what reaches it.
 static int tk_blocks(int rows, int V, int k) {
   int blocks = 1;
-  while (blocks < SEL_BLOCKS && rows * (blocks * 2) <= 4 * 148 && V >= 2048 * (blocks * 2) && k * blocks * 4 <= SEL_CAP) blocks *= 2;
+  while (blocks < SEL_BLOCKS && rows * (blocks * 2) <= 4 * 148 && V >= 2048 * (blocks * 2) && k * 3 <= SEL_CAP) blocks *= 2;
   return blocks;
 }
 
