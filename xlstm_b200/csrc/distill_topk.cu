@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
         count += 1 - old;
       }
     }
+    __syncwarp();   // (see block_reduce)
     if (LOSS) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
       if (LOSS && !CAP) en.z[k] = Z(en.z[k]);
       double e = 0.0;
       if (en.id[k] >= 0 && live) {
-        e = exp(en.t[k] - L);
+        const double d = en.t[k] - L;
+        e = d < -690.0 ? 0.0 : d <= 0.0 ? exp64(d) : exp(d);   // (above 0: a teacher's sum that is not the sum)
         if (LOSS && !(e == 0.0)) F += e * (en.t[k] - (double)en.z[k] * DT_LN2);
       }
       en.e[k] = (float)e;
@@ -218,6 +220,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
         if (first) sS += exp2_approx(en.z[k] - mS);
       }
     }
+    __syncwarp();
     if (LOSS) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -277,6 +280,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
       f2_unpack(f2_add(acc[0], acc[1]), a0, a1);
       sR += a0 + a1;
     }
+    __syncwarp();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sR += __shfl_xor_sync(0xffffffffu, sR, o);
     int all_small = __syncthreads_and(small);   // (and the maximum in s.wf[0] has been read)
@@ -295,6 +299,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
       sR = dt_exchange(sR, s.from[0], rank, blocks, OpSum());
     }
     if (warp == 0) {
+      __syncwarp();
       if (blocks > 1) {
         sS = 0.f;
         for (int r = 0; r < blocks; ++r) { sS += s.from[1][r]; all_small = all_small && s.from[3][r] > 0.f; }
@@ -305,21 +310,22 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
       // sums in one scale, and the four logarithms in four lanes
       const float top = BOUNDED ? 0.f : sR > 0.f ? (sS > 0.f ? fmaxf(mR, mS) : mR) : mS;
       const double tR = BOUNDED || sR == 0.f ? sR : sR * exp2_approx(mR - top), tS = BOUNDED || sS == 0.f ? sS : sS * exp2_approx(mS - top);
-      const double lg = log2(lane == 0 ? (double)sR : lane == 1 ? tR + tS : lane == 2 ? E : left);
+      const double lg = log2_64(lane == 0 ? (double)sR : lane == 1 ? tR + tS : lane == 2 ? E : left);
       const double lR = __shfl_sync(0xffffffffu, lg, 0) + (double)mR, l = __shfl_sync(0xffffffffu, lg, 1) + (double)top;   // log2(0) = -inf
       const double lE = __shfl_sync(0xffffffffu, lg, 2), lleft = __shfl_sync(0xffffffffu, lg, 3);
       if (lane == 0) {
         double loss = 0.0, W = 0.0;
+        const double r = (double)(1.f / (float)E), iE = fma(r, fma(-E, r, 1.0), r);   // 1 / E
         if (live) {
           W = given ? E + left : 1.0;
-          loss = given ? F + E * (l * DT_LN2 - L) : F / E + (l - lE) * DT_LN2 - L;
+          loss = given ? F + E * (l * DT_LN2 - L) : F * iE + (l - lE) * DT_LN2 - L;
           if (!(left == 0.0)) loss += left * (lleft - lR + l) * DT_LN2;
         }
         s.lR = sR == 0.f ? 0.f : (float)lR;
         s.l = (float)l;
-        s.B = sR == 0.f ? 0.f : (float)(W * (tR / (tR + tS)) - left);
+        s.B = sR == 0.f ? 0.f : (float)(W * (double)((float)tR / (float)(tR + tS)) - left);
         s.W = (float)W;
-        s.pscale = given ? 1.f : (float)(1.0 / E);
+        s.pscale = given ? 1.f : (float)iE;
         if (rank == 0) {
           p.loss[row] = (float)((double)p.temperature * (double)p.temperature * loss);
           if (st) {

@@ -44,6 +44,7 @@ template <> struct VocabKey<__nv_bfloat16> {   // the fp32 key's lower half says
 // reductions over a block of WARPS full warps; `s` is shared memory of WARPS elements.  Every thread gets the result.
 // ---------------------------------------------------------------------------------------------
 template <int WARPS, typename V, typename F> __device__ __forceinline__ V block_reduce(V v, F f, V* s) {
+  __syncwarp();   // shuffles of a warp whose lanes have not met again take some 200 cycles each, of one whose have 30
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   __syncthreads();   // (the last use of `s` is over)
@@ -60,6 +61,44 @@ struct OpMax {
 struct OpSum {
   template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
+
+// ---------------------------------------------------------------------------------------------
+// 64-bit arithmetic with short chains: the result of a 64-bit instruction takes some forty cycles
+// ---------------------------------------------------------------------------------------------
+// Conversions between 64-bit numbers and integers or fp32 go through the slowest unit of the SM; here they are bit moves and
+// additions of powers of two.
+__device__ __forceinline__ double double_of(float v) {   // (what is below 2^-126 counts as 0)
+  const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
+  return m < 0x00800000u ? 0.0 : __hiloint2double((int)((b & 0x80000000u) | ((m >> 3) + 0x38000000u)), (int)(m << 29));
+}
+// e^x for x <= 0 (below -700: e^-700): 2^n times the Taylor series of 2^f, |f| <= 1/2, to degree 10: relative error 3e-13
+__device__ __forceinline__ double exp64(double x) {
+  constexpr double LOG2E_64 = 1.4426950408889634, ROUND = 6755399441055744.0;   // 1.5 * 2^52: adding it rounds to whole numbers
+  x = x > -700.0 ? x : -700.0;
+  const double r = fma(x, LOG2E_64, ROUND), f = fma(x, LOG2E_64, ROUND - r);
+  const double f2 = f * f, f4 = f2 * f2;   // (in halves of halves: a chain of five instead of ten)
+  const double p0 = fma(fma(0.05550410866482158, f, 0.24022650695910072), f2, fma(0.6931471805599453, f, 1.0));
+  const double p1 = fma(fma(1.5252733804059841e-05, f, 0.0001540353039338161), f2, fma(0.0013333558146428443, f, 0.009618129107628477));
+  const double p2 = fma(7.054911620801123e-09, f2, fma(1.01780860092397e-07, f, 1.321548679014431e-06));
+  const double p = fma(fma(p2, f4, p1), f4, p0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20), __double2loint(p));   // (exponent >= -1010: no subnormal)
+}
+// 1 / d, 1 <= d <= 2: a Newton step from the fp32 reciprocal (2^-22 squared)
+__device__ __forceinline__ double inverse64(double d) {
+  const uint32_t hi = (uint32_t)__double2hiint(d), lo = (uint32_t)__double2loint(d);
+  const float f = hi >= 0x40000000u ? 2.f : __uint_as_float(0x3f800000u | (hi & 0x000fffffu) << 3 | lo >> 29);
+  const double r = double_of(__fdividef(1.f, f));
+  return fma(r, fma(-d, r, 1.0), r);
+}
+// log2(x) of x >= 0: the fp32 logarithm of the mantissa, and what e^x says is missing from it (error 1e-13)
+__device__ __forceinline__ double log2_64(double x) {
+  if (!(x > 0.0) || x > 1.7e308) return x == 0.0 ? -(double)INFINITY : x;   // (NaN, infinity; not of negative numbers)
+  const int hi = __double2hiint(x), e = (hi >> 20) - 1023;
+  const double m = __hiloint2double((hi & 0x000fffff) | 0x3ff00000, __double2loint(x));
+  const float l = log2f((float)m);
+  const double missing = fma(m, exp64((double)l * -0.69314718055994530942), -1.0);
+  return fma(missing, 1.4426950408889634, (double)l) + (double)e;
+}
 
 // ---------------------------------------------------------------------------------------------
 // fp32 arithmetic of the capped logits, two elements to an instruction

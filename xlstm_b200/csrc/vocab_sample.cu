@@ -24,37 +24,12 @@ constexpr int VS_VALUES = 4096;   // distinct bf16 values of a row that the coun
 constexpr double VS_ONE = 17592186044416.0;   // 2^44
 typedef unsigned long long u64;
 
-// Conversions between 64-bit numbers and integers or fp32 go through the slowest unit of the SM; here they are bit moves and
-// additions of powers of two.
-__device__ __forceinline__ double vs_double(float v) {   // (what is below 2^-126 counts as 0)
-  const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
-  return m < 0x00800000u ? 0.0 : __hiloint2double((int)((b & 0x80000000u) | ((m >> 3) + 0x38000000u)), (int)(m << 29));
-}
+// (64-bit conversions go through the slowest unit of the SM: see vocab_row.cuh)
 __device__ __forceinline__ u64 vs_whole(double w) {   // rint(w 2^44), 0 <= w <= 1
   return (u64)__double_as_longlong(fma(w, VS_ONE, 4503599627370496.0)) & 0x000fffffffffffffull;
 }
 __device__ __forceinline__ double vs_number(u64 m) {   // m < 2^63
   return fma((double)(int)(m >> 32), 4294967296.0, (double)(uint32_t)m);
-}
-
-// e^x for x <= 0: 2^n times the Taylor series of 2^f, |f| <= 1/2, to degree 10: relative error 3e-13, a tenth of the unit of the sums
-__device__ __forceinline__ double vs_exp(double x) {
-  constexpr double LOG2E_64 = 1.4426950408889634, ROUND = 6755399441055744.0;   // 1.5 * 2^52: adding it rounds to whole numbers
-  x = x > -700.0 ? x : -700.0;
-  const double r = fma(x, LOG2E_64, ROUND), f = fma(x, LOG2E_64, ROUND - r);
-  const double f2 = f * f, f4 = f2 * f2;   // (in halves of halves: a chain of five instead of ten)
-  const double p0 = fma(fma(0.05550410866482158, f, 0.24022650695910072), f2, fma(0.6931471805599453, f, 1.0));
-  const double p1 = fma(fma(1.5252733804059841e-05, f, 0.0001540353039338161), f2, fma(0.0013333558146428443, f, 0.009618129107628477));
-  const double p2 = fma(7.054911620801123e-09, f2, fma(1.01780860092397e-07, f, 1.321548679014431e-06));
-  const double p = fma(fma(p2, f4, p1), f4, p0);
-  return __hiloint2double(__double2hiint(p) + (__double2loint(r) << 20), __double2loint(p));   // (exponent >= -1010: no subnormal)
-}
-// 1 / d, 1 <= d <= 2: a Newton step from the fp32 reciprocal (2^-22 squared)
-__device__ __forceinline__ double vs_inverse(double d) {
-  const uint32_t hi = (uint32_t)__double2hiint(d), lo = (uint32_t)__double2loint(d);
-  const float f = hi >= 0x40000000u ? 2.f : __uint_as_float(0x3f800000u | (hi & 0x000fffffu) << 3 | lo >> 29);
-  const double r = vs_double(__fdividef(1.f, f));
-  return fma(r, fma(-d, r, 1.0), r);
 }
 
 // what a row's tokens weigh
@@ -63,8 +38,8 @@ struct VsWeights {
   float largest;
   __device__ __forceinline__ double capped(float v) const {
     if (!(cap > 0.0)) return (double)v;
-    const double e = vs_exp(-2.0 * vs_double(fabsf(v)) * icap);
-    const double y = cap * (1.0 - e) * vs_inverse(1.0 + e);
+    const double e = exp64(-2.0 * double_of(fabsf(v)) * icap);
+    const double y = cap * (1.0 - e) * inverse64(1.0 + e);
     return v < 0.f ? -y : y;
   }
   __device__ __forceinline__ void set(double cap_, double icap_, double invT_, float largest_) {
@@ -72,16 +47,17 @@ struct VsWeights {
     icap = icap_;
     invT = invT_;
     largest = largest_;
-    ymax = capped(largest_);
   }
+  __device__ __forceinline__ void set_max() { ymax = capped(largest); }
   __device__ __forceinline__ double of(float v, double y) const {
-    const double w = vs_exp((y - ymax) * invT);
+    const double w = exp64((y - ymax) * invT);
     return v == largest ? 1.0 : !(v > -INFINITY) || largest == INFINITY ? 0.0 : w;   // 0: NaN and -inf; next to +inf
   }
   __device__ __forceinline__ double of(float v) const { return of(v, capped(v)); }
-  // several at a time: a 64-bit instruction's result takes some forty cycles
-  template <int M> __device__ __forceinline__ void of(const float (&v)[M], double (&out)[M]) const {
+  // several at a time, the largest's cap among them: a 64-bit instruction's result takes some forty cycles
+  template <int M> __device__ __forceinline__ void of(const float (&v)[M], double (&out)[M]) {
     double y[M];
+    set_max();
 #pragma unroll
     for (int i = 0; i < M; ++i) y[i] = capped(v[i]);
 #pragma unroll
@@ -134,6 +110,7 @@ template <int THREADS> __device__ void vs_scan(VsScan<THREADS>& s, unsigned int&
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned int ic = c;
   u64 im = m;
+  __syncwarp();   // (see block_reduce)
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned int oc = __shfl_up_sync(0xffffffffu, ic, o);
@@ -280,6 +257,8 @@ struct VsCounts {
   unsigned int value[VS_VALUES];     // pattern << 16 | count, in order of descending value
   unsigned int group[256];           // non-empty bins of 256 patterns each, in that order; then those in front
   unsigned int values, counted;
+  int last;                          // values of weight min_p and more
+  u64 over;                          // their mass
   VsPlace place;
 };
 
@@ -301,7 +280,7 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat1
   };
   load(tid);
   for (int i = tid; i < 8192; i += THREADS) reinterpret_cast<uint4*>(s.pair)[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (tid == 0) s.counted = 0u;
+  if (tid == 0) { s.counted = 0u; s.last = 0; }
   __syncthreads();
   auto count = [&](uint32_t bits) { atomicAdd(&s.pair[bits >> 1], bits & 1u ? 0x10000u : 1u); };
 #pragma unroll 1
@@ -344,6 +323,7 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat1
   for (int i = 0; i < ROUNDS; ++i) {
     const uint4 u = mine[i];
     unsigned int n = 0u;
+    __syncwarp();
     if (__any_sync(0xffffffffu, (u.x | u.y | u.z | u.w) != 0u)) {
       n = __reduce_add_sync(0xffffffffu, __popc(filled(u, unit_of(i * WARPS + warp))));
       sum += (u.x & 0xffffu) + (u.x >> 16) + (u.y & 0xffffu) + (u.y >> 16) + (u.z & 0xffffu) + (u.z >> 16) + (u.w & 0xffffu) + (u.w >> 16);
@@ -351,6 +331,7 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat1
     if (lane == 0) s.group[i * WARPS + warp] = n;
   }
   if (V > 65535) {
+    __syncwarp();
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == 0) atomicAdd(&s.counted, sum);
   }
@@ -360,6 +341,7 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat1
 #pragma unroll
     for (int i = 0; i < 8; ++i) n += c[i] = s.group[8 * lane + i];
     unsigned int upto = n;
+    __syncwarp();
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -376,9 +358,11 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat1
   for (int i = 0; i < ROUNDS; ++i) {
     const int g = i * WARPS + warp, unit = unit_of(g);
     const uint4 u = mine[i];
+    __syncwarp();
     if (!__any_sync(0xffffffffu, (u.x | u.y | u.z | u.w) != 0u)) continue;
     const unsigned int m = filled(u, unit), n = __popc(m);
     unsigned int upto = n;
+    __syncwarp();
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -397,12 +381,15 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat1
   return true;
 }
 
+// The weights by all threads; the scan and the questions by the first 256 only: shuffles and barriers of 32 warps take longer than
+// a few more additions a thread (a scan of masses over 1024 threads: 2 000 cycles).
+constexpr int VS_FIRST = 256;
+__device__ __forceinline__ void vs_first_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(VS_FIRST) : "memory"); }
+
 template <int THREADS>
-__device__ VsPlace vs_counted_sample(VsCounts& s, VsScan<THREADS>& scan, const VsWeights& w, const VsSettings& set) {
-  const int tid = threadIdx.x, values = (int)s.values, per = (values + THREADS - 1) / THREADS, i0 = min(values, tid * per), i1 = min(values, i0 + per);
-  auto key_of = [](uint32_t e) { return VocabKey<__nv_bfloat16>::of(__ushort_as_bfloat16((unsigned short)(e >> 16))); };
-  u64 over = 0ull, mass = 0ull, all, t;
-  unsigned int count = 0u, tc;
+__device__ VsPlace vs_counted_sample(VsCounts& s, VsScan<THREADS>& scan, VsWeights& w, const VsSettings& set, int V) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, values = (int)s.values;
+  int last = 0;   // values of weight min_p and more
 #pragma unroll 1
   for (int i = tid; i < values; i += 3 * THREADS) {
     uint32_t e[3];
@@ -414,54 +401,92 @@ __device__ VsPlace vs_counted_sample(VsCounts& s, VsScan<THREADS>& scan, const V
 #pragma unroll
     for (int h = 0; h < 3; ++h)
       if (i + h * THREADS < values) {
-        const u64 each = VsWeights::whole(v[h]);
-        s.each[i + h * THREADS] = each;
-        if (v[h] >= (double)set.min_p) over += each * (e[h] & 0xffffu);
+        s.each[i + h * THREADS] = VsWeights::whole(v[h]);
+        if (v[h] >= (double)set.min_p) last = i + h * THREADS + 1;
       }
+  }
+  if (set.min_p > 0.f) {
+    __syncwarp();
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0 && last) atomicMax(&s.last, last);
   }
   __syncthreads();
-  for (int i = i0; i < i1; ++i) { const unsigned int c = s.value[i] & 0xffffu; mass += s.each[i] * c; count += c; }
-  u64 before_m = mass;
-  unsigned int before_c = count;
-  vs_scan<THREADS>(scan, before_c, before_m, &tc, &all);
-  // (the thread that has the place works it out)
-  auto find = [&](bool by_mass, u64 goal) {
-    const u64 lo = by_mass ? before_m : before_c, hi = lo + (by_mass ? mass : count);
-    if (lo < goal && goal <= hi) {
-      u64 m = before_m;
-      unsigned int c = before_c;
-      for (int i = i0;; ++i) {
-        const unsigned int bc = s.value[i] & 0xffffu;
-        const u64 each = s.each[i], bm = each * bc;
-        if (goal <= (by_mass ? m + bm : (u64)(c + bc))) {
-          s.place.key = key_of(s.value[i]);
-          s.place.rank = by_mass ? vs_steps(goal - m, each) - 1u : (unsigned int)(goal - c) - 1u;
-          s.place.upto = m + (u64)(s.place.rank + 1u) * each;
-          break;
-        }
-        m += bm;
-        c += bc;
-      }
+  if (tid < VS_FIRST) {
+    const int per = (values + VS_FIRST - 1) / VS_FIRST, i0 = min(values, tid * per), i1 = min(values, i0 + per);
+    u64 mass = 0ull, over = 0ull;
+    unsigned int count = 0u;
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) {
+      const unsigned int c = s.value[i] & 0xffffu;
+      mass += s.each[i] * c;
+      count += c;
+      if (i < s.last) over = mass;
     }
-    __syncthreads();
-    const VsPlace r = s.place;
-    __syncthreads();
-    return r;
-  };
-  u64 kept = all;
-  if (set.top_k < (int)tc) kept = find(false, (u64)set.top_k).upto;   // (NaN is not counted here: fewer tokens than top_k are all kept)
-  const u64 one = (u64)VS_ONE;
-  if (set.top_p < 1.f) {
-    const double goal = set.top_p_goal(kept);
-    kept = goal > 1.0 ? find(true, min((u64)goal, kept)).upto : one;
+    // masses and counts in front of this thread's values, and their sums
+    u64 before_m = mass;
+    unsigned int before_c = count;
+    __syncwarp();
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 om = __shfl_up_sync(0xffffffffu, before_m, o);
+      const unsigned int oc = __shfl_up_sync(0xffffffffu, before_c, o);
+      if (lane >= o) { before_m += om; before_c += oc; }
+    }
+    if (lane == 31) { scan.m[warp] = before_m; scan.c[warp] = before_c; }
+    vs_first_barrier();
+    u64 all = 0ull;
+    unsigned int tc = 0u;
+    before_m -= mass;
+    before_c -= count;
+#pragma unroll
+    for (int i = 0; i < VS_FIRST / 32; ++i) {
+      if (i < warp) { before_m += scan.m[i]; before_c += scan.c[i]; }
+      all += scan.m[i];
+      tc += scan.c[i];
+    }
+    if (set.min_p > 0.f && i0 < s.last && s.last <= i1) s.over = before_m + over;
+    // one prefix question; the thread that has the place works it out
+    auto find = [&](bool by_mass, u64 goal) {
+      const u64 lo = by_mass ? before_m : before_c, hi = lo + (by_mass ? mass : count);
+      if (lo < goal && goal <= hi) {
+        u64 m = before_m;
+        unsigned int c = before_c;
+#pragma unroll 2
+        for (int i = i0;; ++i) {
+          const unsigned int bc = s.value[i] & 0xffffu;
+          const u64 each = s.each[i], bm = each * bc;
+          if (goal <= (by_mass ? m + bm : (u64)(c + bc))) {
+            s.place.key = VocabKey<__nv_bfloat16>::of(__ushort_as_bfloat16((unsigned short)(s.value[i] >> 16)));
+            s.place.rank = by_mass ? vs_steps(goal - m, each) - 1u : (unsigned int)(goal - c) - 1u;
+            s.place.upto = m + (u64)(s.place.rank + 1u) * each;
+            break;
+          }
+          m += bm;
+          c += bc;
+        }
+      }
+      vs_first_barrier();
+      const u64 upto = s.place.upto;
+      vs_first_barrier();
+      return upto;
+    };
+    u64 kept = all;
+    if (set.top_k < V && set.top_k < (int)tc) kept = find(false, (u64)set.top_k);   // (NaN is not counted here: fewer tokens than top_k are all kept)
+    const u64 one = (u64)VS_ONE;
+    if (set.top_p < 1.f) {
+      const double goal = set.top_p_goal(kept);
+      kept = goal > 1.0 ? find(true, min((u64)goal, kept)) : one;
+    }
+    if (set.min_p > 0.f) {
+      vs_first_barrier();   // (s.over)
+      kept = min(kept, s.last ? s.over : 0ull);
+    } else if (!(set.min_p <= 0.f)) {
+      kept = 0ull;   // (NaN: nothing but the first token)
+    }
+    find(true, set.goal(max(one, kept)));
   }
-  if (!(set.min_p <= 0.f)) {
-    unsigned int none = 0u;
-    vs_scan<THREADS>(scan, none, over, &tc, &t);
-    kept = min(kept, t);
-  }
-  kept = max(one, kept);
-  return find(true, set.goal(kept));
+  __syncthreads();
+  return s.place;
 }
 
 // places of a vector's elements that equal v, as bits (-0 equals +0)
@@ -499,6 +524,7 @@ template <typename T, int THREADS> __device__ void vs_locate(unsigned int* wc, c
     n += __popc(kept[i]);
   }
   for (int v = v0 + 32 * KEEP + lane; v < v1; v += 32) n += __popc(vs_equal<T>(__ldg(xv + v), value));
+  __syncwarp();
   n = __reduce_add_sync(0xffffffffu, n);
   __syncthreads();
   if (lane == 0) wc[warp] = n;
@@ -511,25 +537,39 @@ template <typename T, int THREADS> __device__ void vs_locate(unsigned int* wc, c
     if (hit && before + __popc(mask & ((1u << lane) - 1u)) == rank) *out = j0 + lane;
     before += __popc(mask);
   };
-  auto round = [&](unsigned int m, int v) {
-    const unsigned int sum = __reduce_add_sync(0xffffffffu, __popc(m));
-    if (rank < before + sum && rank >= before) {   // here
-      unsigned int upto = __popc(m);
+  // the round of 32 vectors that has the token, from the counts of all at once
+  auto inside = [&](unsigned int m, int v) {
+    unsigned int upto = __popc(m);
+    __syncwarp();
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned int c = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += c;
-      }
-      unsigned int at = before + upto - __popc(m);
-      for (unsigned int b = m; b; b &= b - 1u, ++at)
-        if (at == rank) *out = slice.element(v + lane) + __ffs(b) - 1;
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned int c = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += c;
     }
-    before += sum;
+    unsigned int at = before + upto - __popc(m);
+    for (unsigned int b = m; b; b &= b - 1u, ++at)
+      if (at == rank) *out = slice.element(v + lane) + __ffs(b) - 1;
   };
   if (warp == 0) single(0, slice.head);
+  if (rank < before) return;
+  unsigned int sums[KEEP];
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < KEEP; ++i) round(kept[i], v0 + 32 * i);
-  for (int v = v0 + 32 * KEEP; v < v1; v += 32) round(v + lane < v1 ? vs_equal<T>(__ldg(xv + v + lane), value) : 0u, v);
+  for (int i = 0; i < KEEP; ++i) sums[i] = __reduce_add_sync(0xffffffffu, __popc(kept[i]));
+  unsigned int m = 0u;
+  int at = -1;
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) {
+    if (at < 0 && rank < before + sums[i]) { at = i; m = kept[i]; }
+    if (at < 0) before += sums[i];
+  }
+  if (at >= 0) { inside(m, v0 + 32 * at); return; }
+  for (int v = v0 + 32 * KEEP; v < v1; v += 32) {
+    m = v + lane < v1 ? vs_equal<T>(__ldg(xv + v + lane), value) : 0u;
+    const unsigned int sum = __reduce_add_sync(0xffffffffu, __popc(m));
+    if (rank < before + sum) { inside(m, v); return; }
+    before += sum;
+  }
   if (warp == WARPS - 1) single(tail, V);
 }
 
@@ -597,6 +637,7 @@ template <typename T, int THREADS> __device__ void vs_greedy(const T* x, int V, 
     const float y = cap > 0.f ? capped_rounded<T>(x[j], cap) : to_float(x[j]);
     if (y > bv || (y == bv && j < bi)) { bv = y; bi = j; }
   }
+  __syncwarp();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
@@ -636,6 +677,7 @@ template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(T
   VsWeights w;
   auto weigh = [&](float largest) {
     w.set(p.cap, icap, invT, largest);
+    w.set_max();
   };
   VsPlace place;
   bool found = false;
@@ -657,6 +699,7 @@ template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(T
           const int step = shift < 5 ? shift : 5, lane = threadIdx.x & 31;
           shift -= step;
           const uint32_t mine = key | (uint32_t)lane << shift | ((1u << shift) - 1u);   // the largest key of the lane's stretch
+          __syncwarp();
           const bool in = lane >> step == 0 && (mine >= kmax || w.of(VocabKey<T>::value(mine)) >= (double)set.min_p);
           const unsigned int some = __ballot_sync(0xffffffffu, in);
           key |= (uint32_t)(some ? __ffs(some) - 1 : 0) << shift;
@@ -681,8 +724,8 @@ template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(T
         if (threadIdx.x == 0) p.tokens[row] = 0;
         return;
       }
-      weigh(largest);
-      place = vs_counted_sample<THREADS>(s, scan, w, set);
+      w.set(p.cap, icap, invT, largest);
+      place = vs_counted_sample<THREADS>(s, scan, w, set, p.V);
       found = true;
     } else if (!few && !alone) {   // (the digits need the largest logit)
       Selector<T, THREADS, 0> sel(ss, x, p.V, 0, 1);

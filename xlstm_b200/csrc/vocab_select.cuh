@@ -113,6 +113,7 @@ template <int STEP, int BATCH, typename F> __device__ __forceinline__ void for_v
 // a warp's 32 values in descending order over its lanes
 template <typename V> __device__ __forceinline__ V run_sorted(V e) {
   const int lane = threadIdx.x & 31;
+  __syncwarp();
 #pragma unroll
   for (int len = 2; len <= 32; len <<= 1)
 #pragma unroll
@@ -179,11 +180,13 @@ template <typename T, int THREADS, int KEEP> struct Selector {
     const bool both = groups < 2 * THREADS;
     if (both) ge = max(ge, go);
     const int share = both ? THREADS / groups : 1;   // threads of a group
+    __syncwarp();
     for (int o = 1; o < share; o <<= 1) ge = max(ge, __shfl_xor_sync(0xffffffffu, ge, o));
     if (k > 1 && tid % share == 0) {
       s.group[tid / share] = (unsigned short)ge;
       if (!both) s.group[THREADS + tid] = (unsigned short)go;
     }
+    __syncwarp();
     const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of_float(fmaxf(g.even(), g.odd())));
     if (lane == 0) s.largest[tid >> 5] = mine;
     if (tid == 0) s.n = s.mine = 0u;
@@ -232,6 +235,7 @@ template <typename T, int THREADS, int KEEP> struct Selector {
       lo = min(lo, min(key[2 * i], key[2 * i + 1]));
       hi = max(hi, max(key[2 * i], key[2 * i + 1]));
     }
+    __syncwarp();
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
     uint32_t bit = lo == hi ? 0u : 0x80000000u >> __clz(lo ^ hi), t = bit ? hi & ~(2u * bit - 1u) : hi;
@@ -334,6 +338,7 @@ template <typename T, int THREADS> __device__ __noinline__ void select_exact(Sel
     unsigned int sum = 0u;
     for (int i = 0; i < PER; ++i) sum += b0 - i >= 0 ? s.count[b0 - i] : 0u;
     unsigned int upto = sum;
+    __syncwarp();
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -364,6 +369,7 @@ template <typename T, int THREADS> __device__ __noinline__ void select_exact(Sel
     if (key > prefix) list[atomicAdd(&s.n, 1u)] = entry(key, j);
     n += key == prefix;
   }
+  __syncwarp();
   n = __reduce_add_sync(0xffffffffu, n);
   if (lane == 0) s.wc[warp] = n;
   __syncthreads();

@@ -13,7 +13,7 @@ template <int THREADS> struct TkShared {
   float wf[THREADS / 32], from[SEL_BLOCKS];
 };
 
-template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> __global__ void __launch_bounds__(THREADS, KEEP ? 2 : 1024 / THREADS) topk_kernel(const xl_topk_params p, const CappedZ<CAP> Z0, const int blocks) {
+template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> __global__ void __launch_bounds__(THREADS, KEEP ? 2 : 1024 / THREADS) topk_kernel(const xl_topk_params p, const CappedZ<CAP> Z0, const double invT, const int blocks) {
   __shared__ TkShared<THREADS> s;
   constexpr int N = Vec16<T>::N;
   const int tid = threadIdx.x, k = p.k, rank = blocks > 1 ? (int)cluster_ctarank() : 0;
@@ -70,7 +70,7 @@ template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> __global__ 
       sum = s.from[0];
       for (int r = 1; r < blocks; ++r) sum += s.from[r];
     }
-    p.lse[row] = isinf(largest) && !CAP ? largest : (float)((log2((double)sum) + (double)zmax) * 0.69314718055994530942 + (CAP ? 0.0 : (double)Z.ref / (double)p.temperature));
+    p.lse[row] = isinf(largest) && !CAP ? largest : (float)((log2_64((double)sum) + (double)zmax) * 0.69314718055994530942 + (CAP ? 0.0 : (double)Z.ref * invT));
   }
   if (n > SEL_CAP || n < (unsigned int)k) {
     select_exact<T, THREADS>(s.exact, s.sel.list, x, p.V, k);
@@ -104,7 +104,7 @@ template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> static int 
   attr[0].val.clusterDim = {(unsigned)blocks, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, topk_kernel<T, CAP, BOUNDED, THREADS, KEEP>, *p, CappedZ<CAP>(p->cap, p->temperature), blocks));
+  XL_CUDA_TRY(cudaLaunchKernelEx(&cfg, topk_kernel<T, CAP, BOUNDED, THREADS, KEEP>, *p, CappedZ<CAP>(p->cap, p->temperature), 1.0 / (double)p->temperature, blocks));
   return check_launch("xl_softcap_topk");
 }
 
