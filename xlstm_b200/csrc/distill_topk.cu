@@ -61,13 +61,17 @@ struct No { static constexpr bool value = false; };
 
 // f(vector, its number) for v, v + STEP, .. below end, four loads under way at a time
 template <int STEP, typename F> __device__ __forceinline__ void dt_vectors(const uint4* xv, int v, int end, F f) {
+  const int over = 31 - (int)(threadIdx.x & 31) + 3 * STEP;
 #pragma unroll 1
-  for (; v + 3 * STEP < end; v += 4 * STEP) {
+  for (; v + over < end; v += 4 * STEP) {   // (all lanes together: f may part them)
     uint4 u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) u[i] = __ldg(xv + v + i * STEP);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f(u[i], v + i * STEP);
+    for (int i = 0; i < 4; ++i) {
+      f(u[i], v + i * STEP);
+      __syncwarp();
+    }
   }
 #pragma unroll 1
   for (; v < end; v += STEP) f(__ldg(xv + v), v);

@@ -98,16 +98,20 @@ template <> __device__ __forceinline__ float vec_element<float>(const uint4& u, 
 
 // f(vector, its number) for v, v + STEP, .. below end, BATCH loads under way at a time
 template <int STEP, int BATCH, typename F> __device__ __forceinline__ void for_vectors(const uint4* xv, int v, int end, F f) {
+  const int over = 31 - (int)(threadIdx.x & 31) + (BATCH - 1) * STEP;   // of the warp's last lane in the batch's last round
 #pragma unroll 1
-  for (; v < end; v += BATCH * STEP) {
+  for (; v + over < end; v += BATCH * STEP) {   // (all lanes together: f may part them)
     uint4 u[BATCH];
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i)
-      if (v + i * STEP < end) u[i] = __ldg(xv + v + i * STEP);
+    for (int i = 0; i < BATCH; ++i) u[i] = __ldg(xv + v + i * STEP);
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i)
-      if (v + i * STEP < end) f(u[i], v + i * STEP);
+    for (int i = 0; i < BATCH; ++i) {
+      f(u[i], v + i * STEP);
+      __syncwarp();
+    }
   }
+#pragma unroll 1
+  for (; v < end; v += STEP) f(__ldg(xv + v), v);
 }
 
 // a warp's 32 values in descending order over its lanes
