@@ -277,6 +277,24 @@ def test_distill_long_rows(tag, V):
     _check_distill(x, values, ids, None, 1.0, None, None)
 
 
+@pytest.mark.parametrize("cap", [0.05, 0.125, 1024.0, 5e4])
+def test_caps_of_every_size(cap):
+    """Logits below, near and far beyond the cap; caps whose powers leave fp32."""
+    import xlstm_b200
+    g = torch.Generator().manual_seed(40)
+    for scale in (0.1, 0.6, 2.0, 30.0):
+        x = cap * scale * torch.randn(4, 3001, generator=g)
+        T = max(1e-2, cap * 0.1)          # (weights spread over a few hundred tokens)
+        _check_sample(x, cap, torch.rand(4, generator=g), T=T, p=0.9)
+        values, ids, lse = _teacher(g, x, 16, cap, T, True)
+        _check_distill(x, values, ids, cap, T, lse, None)
+        got, at, total = xlstm_b200.softcap_topk(x.cuda(), cap, 20, T)
+        for r in range(4):
+            y, idx, l = O.topk_row(x[r], cap, 20, T)
+            assert at[r].tolist() == idx and ((got[r].cpu().double() - y).abs() <= 8 * E24 * y.abs()).all()
+            assert abs(float(total[r]) - float(l)) <= _rel(float((O.cap64(x[r], cap) / T).abs().max())) + 64 * E24 + E24 * abs(float(l))
+
+
 @pytest.mark.parametrize("tag", ["bf16", "f32"])
 def test_distill_extremes(tag):
     """Tokens named twice and often, masked student tokens, entries without mass, far-away tails, all tokens named."""

@@ -184,12 +184,24 @@ template <> struct Vec16<float> {
 // near the row's largest logit, so that rows near the type's lowest value (masks) do not overflow.
 template <bool CAP> struct CappedZ {
   float a, icap, ref, flat;   // flat = 1 / a^2: the cap's slope is 1 - flat z^2
+  // z = x Q(x^2) for magnitudes up to `limit`: the polynomial's coefficients with a and the powers of the cap inside, which
+  // saves the product x / cap; for caps outside 1/8 .. 1024, whose powers leave fp32, nothing counts as small
+  float q0, q1, q2, q3, q4, q5, limit;
   CappedZ(float cap, float temperature) {   // (on the host: the constants are kernel parameters)
     const double scale = 1.4426950408889634 / (double)temperature, wide = CAP ? scale * (double)cap : scale;
     a = (float)wide;
     ref = 0.f;
     icap = CAP ? (float)(1.0 / (double)cap) : 0.f;
     flat = CAP ? (float)(1.0 / (wide * wide)) : 0.f;
+    const bool fits = CAP && cap >= 0.125f && cap <= 1024.f;
+    const double i1 = fits ? 1.0 / (double)cap : 0.0, i2 = i1 * i1;
+    q0 = (float)(wide * i1);
+    q1 = (float)(wide * C1 * i1 * i2);
+    q2 = (float)(wide * C2 * i1 * i2 * i2);
+    q3 = (float)(wide * C3 * i1 * i2 * i2 * i2);
+    q4 = (float)(wide * C4 * i1 * i2 * i2 * i2 * i2);
+    q5 = (float)(wide * C5 * i1 * i2 * i2 * i2 * i2 * i2);
+    limit = fits ? TANH_SMALL * cap : -1.f;
   }
   static constexpr float C1 = -0.33332958817481995f, C2 = 0.1332540661096573f, C3 = -0.05334443226456642f, C4 = 0.01958290860056877f, C5 = -0.004716257099062204f;
   __device__ __forceinline__ float operator()(float x) const {
@@ -205,7 +217,7 @@ template <bool CAP> struct CappedZ {
     if (fabsf(z) > TANH_SMALL) return tanh_large(z);
     return z * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, C5, C4), C3), C2), C1), 1.f);
   }
-  __device__ __forceinline__ bool small(float magnitude) const { return !CAP || magnitude * icap <= TANH_SMALL; }
+  __device__ __forceinline__ bool small(float magnitude) const { return !CAP || magnitude <= limit; }
   // of a vector's elements; SMALL: the caller has seen that all magnitudes are small
   template <bool SMALL, typename T> __device__ __forceinline__ void of(const Vec16<T>& v, f32x2 (&out)[Vec16<T>::N / 2]) const {
     if (!CAP) {
@@ -216,12 +228,12 @@ template <bool CAP> struct CappedZ {
     if (SMALL) {
 #pragma unroll
       for (int i = 0; i < Vec16<T>::N / 2; ++i) {
-        const f32x2 z = f2_mul(v.p[i], f2_dup(icap)), s = f2_mul(z, z);
-        f32x2 q = f2_fma(s, f2_dup(a * C5), f2_dup(a * C4));
-        q = f2_fma(s, q, f2_dup(a * C3));
-        q = f2_fma(s, q, f2_dup(a * C2));
-        q = f2_fma(s, q, f2_dup(a * C1));
-        out[i] = f2_mul(z, f2_fma(s, q, f2_dup(a)));
+        const f32x2 x = v.p[i], s = f2_mul(x, x);
+        f32x2 q = f2_fma(s, f2_dup(q5), f2_dup(q4));
+        q = f2_fma(s, q, f2_dup(q3));
+        q = f2_fma(s, q, f2_dup(q2));
+        q = f2_fma(s, q, f2_dup(q1));
+        out[i] = f2_mul(x, f2_fma(s, q, f2_dup(q0)));
       }
       return;
     }
