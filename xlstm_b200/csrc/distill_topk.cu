@@ -287,6 +287,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     __syncwarp();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sR += __shfl_xor_sync(0xffffffffu, sR, o);
+    __syncwarp();
     int all_small = __syncthreads_and(small);   // (and the maximum in s.wf[0] has been read)
     if (lane == 0) s.wf[0][warp] = sR;
     __syncthreads();

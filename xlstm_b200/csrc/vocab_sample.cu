@@ -384,7 +384,10 @@ template <int THREADS> __device__ bool vs_counts(VsCounts& s, const __nv_bfloat1
 // The weights by all threads; the scan and the questions by the first 256 only: shuffles and barriers of 32 warps take longer than
 // a few more additions a thread (a scan of masses over 1024 threads: 2 000 cycles).
 constexpr int VS_FIRST = 256;
-__device__ __forceinline__ void vs_first_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(VS_FIRST) : "memory"); }
+__device__ __forceinline__ void vs_first_barrier() {
+  __syncwarp();   // (whole warps arrive)
+  asm volatile("bar.sync 1, %0;" ::"n"(VS_FIRST) : "memory");
+}
 
 template <int THREADS>
 __device__ VsPlace vs_counted_sample(VsCounts& s, VsScan<THREADS>& scan, VsWeights& w, const VsSettings& set, int V) {

@@ -163,6 +163,7 @@ template <typename T, int THREADS, int KEEP> struct Selector {
   // barrier.
   __device__ void bound(int k) {
     const int tid = threadIdx.x, lane = tid & 31;
+    __syncwarp();
     if (blocks > 1) cluster_arrive();
     GroupMax<T> g;
     if (KEEP) {
