@@ -100,6 +100,59 @@ def test_sample_ties_and_borders(tag):
 
 
 @pytest.mark.parametrize("tag", ["bf16", "f32"])
+def test_sample_long_rows_of_every_kind(tag):
+    """Rows that fill lists, counters and the table of values: ties by the thousand, more tokens kept than a list holds, many
+    distinct values, equal logits beyond 16 bits of count, masks and NaN among them -- few rows (cut over blocks) and several."""
+    g = torch.Generator().manual_seed(14)
+    dt = DT[tag]
+    V = 70003
+    x = _logits(g, 8, V, dt)
+    x[1] = 2.5                                                   # 70 003 equal logits
+    x[2] = torch.randint(-2, 3, (V,), generator=g).to(dt)        # five values
+    x[3] = torch.randint(0, 2 ** 15, (V,), generator=g).to(torch.int16).view(torch.bfloat16).nan_to_num(0.0, 0.0, 0.0).clamp(max=50.0).to(dt)   # thousands of values
+    x[4, 3:] = -math.inf
+    x[5, ::2] = math.nan
+    x[6] = 0.01 * torch.randn(V, generator=g)                    # nearly flat
+    x[7, 40000:] = torch.finfo(dt).min
+    u = torch.rand(8, generator=g)
+    for cap, kw in ((30.0, dict(k=50)), (None, dict(k=50, p=0.9)), (30.0, dict(k=400)), (None, dict(k=5000, p=0.7, mp=0.001)), (30.0, dict(mp=0.9)), (None, dict(mp=1e-6)),
+                    (30.0, dict(p=0.95, T=0.6)), (None, {}), (30.0, dict(k=1)), (30.0, dict(k=256)), (30.0, dict(k=257))):
+        _check_sample(x, cap, u, **kw)
+        _check_sample(x[:2], cap, u[:2], **kw)
+    _check_sample(x[:, :20011], 30.0, u, torch.full((8,), 0.9), torch.tensor([50, 50, 0, 0, 300, 7, 0, 1000]), torch.tensor([1.0, 0.9, 1.0, 0.5, 1.0, 1.0, 0.3, 0.8]),
+                  torch.tensor([0.0, 0.0, 0.5, 0.0, 0.0, 0.1, 0.0, 0.2]))
+
+
+def test_rows_beyond_the_grid_and_elements_beyond_32_bits():
+    import xlstm_b200
+    g = torch.Generator().manual_seed(15)
+    rows = 70001
+    x = torch.randn(rows, 12, generator=g)
+    u = torch.rand(rows, generator=g)
+    pick = [0, 65535, 65536, 70000]
+    got = xlstm_b200.softcap_sample(x.cuda(), None, u.cuda(), top_k=5)
+    _check_sample(x[pick], None, u[pick], k=5, got=got[pick])
+    values, ids, lse = xlstm_b200.softcap_topk(x.cuda(), None, 3)
+    for r in pick:
+        assert ids[r].tolist() == O.topk_row(x[r], None, 3)[1]
+    loss, grad = xlstm_b200.distill_topk_grad(x.cuda(), values, ids)
+    torch.testing.assert_close(loss[pick].cpu().double(), O.distill(x[pick].double(), values[pick].cpu(), ids[pick].cpu()), rtol=1e-5, atol=1e-6)
+    del x, got, grad
+    big = torch.zeros(42800, 50304, dtype=torch.bfloat16, device="cuda")     # 2.15e9 elements
+    tail = _logits(g, 2, 50304, torch.bfloat16)
+    big[-2:] = tail.cuda()
+    values, ids, lse = xlstm_b200.softcap_topk(big, 30.0, 8)
+    alone = xlstm_b200.softcap_topk(tail.cuda(), 30.0, 8)
+    assert torch.equal(ids[-2:], alone[1]) and torch.equal(values[-2:], alone[0]) and ids[0].tolist() == list(range(8))
+    loss, grad = xlstm_b200.distill_topk_grad(big, values, ids, None, 30.0, 1.0, lse)
+    one, want = xlstm_b200.distill_topk_grad(tail.cuda(), *alone[:2], None, 30.0, 1.0, alone[2])
+    torch.testing.assert_close(loss[-2:], one, rtol=1e-4, atol=1e-6)
+    torch.testing.assert_close(grad[-2:].float(), want.float(), rtol=2 ** -6, atol=1e-7)   # (another cut of the row: a bf16 step here and there)
+    u = torch.full((42800,), 0.5, device="cuda")
+    assert torch.equal(xlstm_b200.softcap_sample(big, 30.0, u, 0.9, 40)[-2:], xlstm_b200.softcap_sample(tail.cuda(), 30.0, u[:2], 0.9, 40))
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
 def test_sample_masked_rows(tag):
     import xlstm_b200
     dt = DT[tag]
@@ -466,6 +519,25 @@ def test_vocab_operators_on_another_stream_and_in_graphs():
         torch.cuda.synchronize()
         for o in outs:
             assert all(torch.equal(a, b) for a, b in zip(o, want))
+
+
+def test_distill_backward_in_a_graph():
+    """Captured behind an eager pass over the same leaf, whose own graph is gone by then (PyTorch ties a leaf's accumulation node to the
+    stream it was made on and invalidates a capture that meets an older one)."""
+    from xlstm_b200 import ops
+    g = torch.Generator().manual_seed(33)
+    leaf = _logits(g, 4, 3001, torch.float32).cuda().requires_grad_()
+    values, ids, lse = (t.cuda() for t in _teacher(g, leaf.detach().cpu(), 8, 30.0, 1.0, True))
+    want, = torch.autograd.grad(ops.distill_topk(leaf, values, ids, 30.0, 1.0, lse).mean(), leaf)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(ops.distill_topk(leaf, values, ids, 30.0, 1.0, lse).mean(), leaf)
+    got.zero_()
+    graph.replay()
+    assert torch.equal(got, want)
+    ops.distill_topk(leaf, values, ids, 30.0, 1.0, lse).mean().backward()   # and eager again
+    assert torch.equal(leaf.grad, want)
 
 
 def test_vocab_operators_give_the_same_bits_again():

@@ -375,7 +375,7 @@ def softcap_topk(logits, cap: Optional[float], k: int, temperature: float = 1.0)
     """The ``k`` largest soft-capped logits of every row and the row's log-sum-exp: what a teacher leaves for
     :func:`distill_topk`.  Returns ``values`` (..., k) float32 (capped, not divided by the temperature, descending; equal
     logits: lower index first; NaN last), ``ids`` (..., k) int32 and ``lse`` (...) float32, the log of the sum of
-    ``exp(y / temperature)`` over all V.  ``k`` up to 1024."""
+    ``exp(y / temperature)`` over all V.  ``k`` up to 1024.  Not recorded by autograd."""
     return native().softcap_topk(logits, cap, k, temperature)
 
 
@@ -407,7 +407,8 @@ def distill_topk(logits, values, ids, cap: Optional[float] = None, temperature: 
 
     A row without a used entry costs nothing and has gradient 0 (padding).  A token named twice counts with both its
     entries.  Ids beyond V count as unused and are reported by :func:`check_device_status`.  The teacher's tensors get no
-    gradient."""
+    gradient.  A pass captured into a CUDA graph wants no eager graph of the same leaf alive (of any operator: PyTorch ties the
+    leaf's accumulation node to the stream it was made on)."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return DistillFunction.apply(logits, values, ids, cap, temperature, teacher_lse)
     return native().distill_topk(logits, values, ids, None, cap, temperature, teacher_lse, 0)
