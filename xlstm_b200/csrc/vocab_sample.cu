@@ -159,6 +159,16 @@ template <typename T, int THREADS> struct VsRow {
   int V;
   VsWeights w;
 
+  // f of every logit of the row
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    const RowSlice<T> slice(x, V, 0, 1);
+    for_vectors<THREADS, 4>(reinterpret_cast<const uint4*>(x + slice.head), threadIdx.x, slice.vectors, [&](const uint4& u, int) {
+#pragma unroll 1
+      for (int i = 0; i < Vec16<T>::N; ++i) f(vec_element<T>(u, i));
+    });
+    for (int i = threadIdx.x; i < slice.n_single(0, 1); i += THREADS) f(x[slice.single(i, 0)]);
+  }
+
   // one prefix question over a histogram: the bin, from the top, in which the running count (or mass) reaches `goal`
   __device__ void find(const VsHist& h, int bins, bool by_mass, u64 goal, unsigned int base_cnt, u64 base_mass) {
     constexpr int PER = VS_BINS / THREADS;
@@ -185,14 +195,14 @@ template <typename T, int THREADS> struct VsRow {
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += THREADS) { h.count[b] = 0u; h.mass[b] = 0ull; }
     __syncthreads();
-    for (int j = threadIdx.x; j < V; j += THREADS) {
-      const uint32_t key = VocabKey<T>::of(x[j]);
-      if (left < VocabKey<T>::BITS && key >> left != prefix) continue;
+    each([&](T e) {
+      const uint32_t key = VocabKey<T>::of(e);
+      if (left < VocabKey<T>::BITS && key >> left != prefix) return;
       const uint32_t b = (key >> (left - step)) & (uint32_t)(bins - 1);
       atomicAdd(&h.count[b], 1u);
-      const u64 m = VsWeights::whole(w.of(VocabKey<T>::value(key)));
+      const u64 m = VsWeights::whole(w.of(to_float(e)));
       if (m) atomicAdd(&h.mass[b], m);
-    }
+    });
     __syncthreads();
   }
 
@@ -227,10 +237,10 @@ template <typename T, int THREADS> struct VsRow {
     unsigned int none = 0u, tc;
     for (int b = threadIdx.x; b < VS_BINS; b += THREADS) all += s.top.mass[b];
     if (set.min_p > 0.f)
-      for (int j = threadIdx.x; j < V; j += THREADS) {
-        const double v = w.of(to_float(x[j]));
+      each([&](T e) {
+        const double v = w.of(to_float(e));
         if (v >= (double)set.min_p) over += VsWeights::whole(v);
-      }
+      });
     vs_scan<THREADS>(scan, none, all, &tc, &t);
     u64 kept = t;
     if (set.top_k < V) kept = descend(false, (u64)set.top_k).upto;
