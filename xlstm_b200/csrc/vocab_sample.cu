@@ -142,14 +142,22 @@ template <int THREADS> __device__ void vs_scan(VsScan<THREADS>& s, unsigned int&
 }
 
 // ---------------------------------------------------------------------------------------------- digits
-struct VsHist {
-  unsigned int count[VS_BINS];
-  u64 mass[VS_BINS];
+struct VsHist {   // masses in two words: 64-bit additions to shared memory would be loops of compare-and-swap
+  unsigned int count[VS_BINS], low[VS_BINS], high[VS_BINS];
+  __device__ __forceinline__ void clear(int b) { count[b] = low[b] = high[b] = 0u; }
+  __device__ __forceinline__ u64 mass(int b) const { return (u64)high[b] << 32 | low[b]; }
+  __device__ __forceinline__ void add(int b, u64 m, bool counts) {
+    if (counts) atomicAdd(&count[b], 1u);
+    const unsigned int lo = (unsigned int)m;
+    unsigned int hi = (unsigned int)(m >> 32);
+    if (lo && atomicAdd(&low[b], lo) > 0xffffffffu - lo) ++hi;   // (the carry, whatever the order)
+    if (hi) atomicAdd(&high[b], hi);
+  }
 };
 template <int THREADS> struct VsDigits {
   VsHist top, sub;   // leading 11 bits; the bits of the descent at work
-  unsigned int bin, cnt, base_cnt;
-  u64 base_mass, bin_mass;
+  unsigned int bin, base_cnt;
+  u64 base_mass;
 };
 
 template <typename T, int THREADS> struct VsRow {
@@ -158,6 +166,7 @@ template <typename T, int THREADS> struct VsRow {
   const T* x;
   int V;
   VsWeights w;
+  bool counts;   // whether somebody asks for counts
 
   // f of every logit of the row
   template <typename F> __device__ __forceinline__ void each(F f) const {
@@ -176,14 +185,14 @@ template <typename T, int THREADS> struct VsRow {
     unsigned int c = 0u, tc;
     u64 m = 0ull, tm;
     for (int i = 0; i < PER; ++i)
-      if (b0 - i >= 0) { c += h.count[b0 - i]; m += h.mass[b0 - i]; }
+      if (b0 - i >= 0) { c += h.count[b0 - i]; m += h.mass(b0 - i); }
     vs_scan<THREADS>(scan, c, m, &tc, &tm);
     c += base_cnt;
     m += base_mass;
     for (int i = 0; i < PER && b0 - i >= 0; ++i) {
       const unsigned int bc = h.count[b0 - i];
-      const u64 bm = h.mass[b0 - i], before = by_mass ? m : c, end = before + (by_mass ? bm : bc);
-      if (before < goal && goal <= end) { s.bin = (unsigned int)(b0 - i); s.cnt = bc; s.bin_mass = bm; s.base_cnt = c; s.base_mass = m; }
+      const u64 bm = h.mass(b0 - i), before = by_mass ? m : c, end = before + (by_mass ? bm : bc);
+      if (before < goal && goal <= end) { s.bin = (unsigned int)(b0 - i); s.base_cnt = c; s.base_mass = m; }
       c += bc;
       m += bm;
     }
@@ -193,15 +202,13 @@ template <typename T, int THREADS> struct VsRow {
   __device__ __noinline__ void histogram(VsHist& h, int left, int step, uint32_t prefix) {
     const int bins = 1 << step;
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += THREADS) { h.count[b] = 0u; h.mass[b] = 0ull; }
+    for (int b = threadIdx.x; b < bins; b += THREADS) h.clear(b);
     __syncthreads();
     each([&](T e) {
       const uint32_t key = VocabKey<T>::of(e);
       if (left < VocabKey<T>::BITS && key >> left != prefix) return;
       const uint32_t b = (key >> (left - step)) & (uint32_t)(bins - 1);
-      atomicAdd(&h.count[b], 1u);
-      const u64 m = VsWeights::whole(w.of(to_float(e)));
-      if (m) atomicAdd(&h.mass[b], m);
+      h.add((int)b, VsWeights::whole(w.of(to_float(e))), counts);
     });
     __syncthreads();
   }
@@ -220,7 +227,7 @@ template <typename T, int THREADS> struct VsRow {
       prefix = (prefix << step) | s.bin;
       left -= step;
     }
-    const u64 each = s.bin_mass / s.cnt;   // of every token of this key
+    const u64 each = VsWeights::whole(w.of(VocabKey<T>::value(prefix)));   // of every token of this key
     VsPlace r;
     r.key = prefix;
     r.rank = by_mass ? vs_steps(goal - s.base_mass, each) - 1u : (unsigned int)(goal - s.base_cnt) - 1u;
@@ -235,7 +242,7 @@ template <typename T, int THREADS> struct VsRow {
     // the whole row's mass, and what min_p leaves of it
     u64 all = 0ull, over = 0ull, t;
     unsigned int none = 0u, tc;
-    for (int b = threadIdx.x; b < VS_BINS; b += THREADS) all += s.top.mass[b];
+    for (int b = threadIdx.x; b < VS_BINS; b += THREADS) all += s.top.mass(b);
     if (set.min_p > 0.f)
       each([&](T e) {
         const double v = w.of(to_float(e));
@@ -748,7 +755,7 @@ template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(T
     __syncthreads();
   }
   if (!found) {
-    VsRow<T, THREADS> r = {*reinterpret_cast<VsDigits<THREADS>*>(smem), scan, x, p.V, w};
+    VsRow<T, THREADS> r = {*reinterpret_cast<VsDigits<THREADS>*>(smem), scan, x, p.V, w, set.top_k < p.V};
     place = r.sample(set);
   }
   vs_locate<T, THREADS>(scan.c, x, p.V, place.key, place.rank, p.tokens + row);
