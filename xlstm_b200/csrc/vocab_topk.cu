@@ -3,6 +3,10 @@
 // Mathematics.  The cap is strictly increasing, so the order is that of the logits as they come.  Two passes over the row: maxima
 // of groups for a bound of the k-th largest (vocab_select.cuh), then the list of what reaches it together with the sum of
 // 2^(z - z_max) in fp32.  The second pass finds the row in L2, so memory is read once.
+//
+// What bounds it.  Many rows: issue slots and load latency, 16 instructions a logit in both passes (of which the cap's polynomial,
+// exponential and sum are 7.5) at 2.2 instructions a cycle and SM: 4096 rows of 50 304 in bf16, k = 64, take 143 us, where their 412 MB are
+// 63 us of memory.  Few rows: the chain of maxima, bisection, list and sort, 8.5 us for 16 rows, cut over clusters of eight blocks.
 #include "vocab_select.cuh"
 
 namespace xl {
