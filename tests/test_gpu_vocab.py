@@ -168,6 +168,11 @@ def test_sample_masked_rows(tag):
     x[6] = low
     x[7, 100:] = -math.inf
     u = torch.rand(8, generator=g)
+    few = torch.full((3, 30000), -math.inf).to(dt)      # constrained decoding: fewer tokens allowed than top_k
+    few[:, ::2999] = _logits(g, 3, 11, dt)
+    few[1] = low
+    _check_sample(few, 30.0, u[:3], k=50)
+    _check_sample(few, None, u[:3], k=12, p=0.9)
     for cap in (None, 30.0):
         for kw in ({}, dict(k=3), dict(p=0.9, T=0.5), dict(mp=0.3), dict(T=math.inf) if cap is None else {}):
             if "T" in kw and kw["T"] == math.inf:   # (as a number it is refused; a tensor's values are not looked at)

@@ -718,6 +718,11 @@ template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(T
     weigh(largest);
     if (few || alone) {
       float least = sel.least();
+      bool whole = ss.bound == 0u;   // the list has every token that can be chosen
+      if (!(least > -INFINITY)) {    // (fewer than top_k are not masked: those)
+        whole = true;
+        least = VocabKey<T>::BITS == 16 ? -3.3895314e38f : -3.4028235e38f;
+      }
       if (alone) {   // the smallest key of weight min_p, five bits at a time: every lane asks for one of 32
         uint32_t key = 0u;
         const uint32_t kmax = VocabKey<T>::of(from_float<T>(largest));
@@ -735,7 +740,7 @@ template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(T
       sel.collect(least, [](const uint4&, int) {}, [](T) {});
       const unsigned int n = sel.gather();
       if (rank != 0) return;
-      if (n <= SEL_CAP && (alone || n >= (unsigned int)set.top_k || ss.bound == 0u)) {
+      if (n <= SEL_CAP && (alone || whole || n >= (unsigned int)set.top_k)) {
         sort_list<THREADS>(ss.list, (int)n);
         vs_listed_sample<T, THREADS>(scan, ss.list, w, set, (int)n, p.tokens + row);
         return;
