@@ -373,6 +373,11 @@ def test_distill_extremes(tag):
     x[6] += 200.0
     for T, l in ((1.0, lse), (1.0, None), (0.25, None)):
         _check_distill(x, values, ids, None, T, l, None)
+    # the same among long rows, whose slices do not all hold the token
+    xl, il = torch.cat([x] * 260, 1)[:, :10301], ids.clone()
+    il[2:, 3] += 9000
+    il[5, 4] = il[5, 3]
+    _check_distill(xl, values, il, None, 1.0, None, None)
     # every token named: the tail counts as empty whatever the teacher's sum says
     full = torch.arange(40, dtype=torch.int32).repeat(8, 1)
     _check_distill(x[5:], values.new_zeros(3, 40), full[5:], None, 1.0, torch.full((3,), math.log(40.0) + 0.01), None)

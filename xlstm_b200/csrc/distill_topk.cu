@@ -22,14 +22,16 @@ constexpr int DT_WARPS = 8, DT_BLOCKS = 8;   // warps: at most
 // with both directions in one launch the second pass finds more of its row in L1 where fewer rows are under way (265, 247 for 4096 rows)
 __host__ __device__ constexpr int dt_threads(bool both) { return both ? 256 : 128; }
 constexpr double DT_LN2 = 0.69314718055994530942;
-// what a row leaves for its gradient; the last two places hold a double
-enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_SMALL = 4, ST_REF = 5, ST_TEACHER = 6 };
+// what a row leaves for its gradient; ST_FLAGS: 1 if its logits stay below three quarters of the cap, and 2 if a token is named
+// twice; the last two places hold a double
+enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_FLAGS = 4, ST_REF = 5, ST_TEACHER = 6 };
 
 struct DtShared {
   double wd[3][DT_WARPS];
   float wf[2][DT_WARPS], from[4][DT_BLOCKS];   // from: of the row's blocks; a place is written once a launch
   int wi[2][DT_WARPS];
   float lR, l, B, W, pscale;
+  int again;   // a token of the slice is named twice (here, not in a register through the passes)
 };
 // Dynamic shared memory: K entries -- t / T, id (-1: unused), z of the student there, e^(t / T - shift) -- and a bit per token of
 // the slice.
@@ -170,13 +172,14 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
   }
   const bool everything = K >= V && count == V;   // no token is left for the tail
   bool again = any & 2, live = any & 1;
+  if (LOSS && tid == 0) s.again = any & 2;
   double L = 0.0;   // shift of the teacher's exponents; with its own sum, or in the backward pass, the right one from the start
   if (LOSS) {
     live = live && (given || m != -INFINITY);
     if (live) L = given ? (double)p.teacher_lse[row] : m;
   } else {
     live = live && st[ST_W] != 0.f;
-    again = true;   // (not known here)
+    again = (int)st[ST_FLAGS] & 2;
     L = *reinterpret_cast<const double*>(st + ST_TEACHER);
   }
   float mR = 0.f, mS = 0.f;   // shifts of the two sums: their largest z (with a bounded z: none)
@@ -304,15 +307,21 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     if (blocks > 1) {
       if (tid < blocks) {
         st_cluster_f32(mapa_u32(smem_u32(s.from[1] + rank), tid), sS);
-        st_cluster_f32(mapa_u32(smem_u32(s.from[3] + rank), tid), (float)all_small);
+        st_cluster_f32(mapa_u32(smem_u32(s.from[3] + rank), tid), (all_small ? 1.f : 0.f) + (float)s.again);
       }
       sR = dt_exchange(sR, s.from[0], rank, blocks, OpSum());
     }
     if (warp == 0) {
       __syncwarp();
+      int named_twice = s.again;   // in any of the slices
       if (blocks > 1) {
         sS = 0.f;
-        for (int r = 0; r < blocks; ++r) { sS += s.from[1][r]; all_small = all_small && s.from[3][r] > 0.f; }
+        for (int r = 0; r < blocks; ++r) {
+          const int flags_r = (int)s.from[3][r];
+          sS += s.from[1][r];
+          all_small = all_small && (flags_r & 1);
+          named_twice |= flags_r & 2;
+        }
       }
       double E = 0.0, F = 0.0;
       for (int w = 0; w < with; ++w) { E += s.wd[0][w]; F += s.wd[1][w]; }
@@ -339,7 +348,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
         if (rank == 0) {
           p.loss[row] = (float)((double)p.temperature * (double)p.temperature * loss);
           if (st) {
-            st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W; st[ST_SMALL] = all_small ? 1.f : 0.f; st[ST_REF] = Z.ref;
+            st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W; st[ST_FLAGS] = (all_small ? 1.f : 0.f) + (float)named_twice; st[ST_REF] = Z.ref;
             *reinterpret_cast<double*>(st + ST_TEACHER) = given ? L : L + lE * DT_LN2;
           }
         }
@@ -347,7 +356,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     }
   } else {
     if (tid == 0) { s.lR = st[ST_LR]; s.l = st[ST_L]; s.B = st[ST_B]; s.W = st[ST_W]; s.pscale = 1.f; }
-    small = st[ST_SMALL] > 0.f;
+    small = (int)st[ST_FLAGS] & 1;
   }
   if (!GRAD) return;
   __syncthreads();
@@ -410,7 +419,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     const int o = slice.place(id);
     if (o < slice.first || o >= slice.end) continue;
     float pk = en.e[k];
-    if (again) {   // a token named twice: all its entries write the same value
+    if (LOSS ? s.again != 0 : again) {   // a token named twice: all its entries write the same value
       pk = 0.f;
       for (int i = 0; i < K; ++i) pk += en.id[i] == id ? en.e[i] : 0.f;
     }
