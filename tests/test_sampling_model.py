@@ -65,6 +65,31 @@ def test_decoder_draws_the_same_tokens_in_any_company_on_cpu():
         ContinuousDecoder(model, 3).run(prompts, counts, sampling=Sampling())
 
 
+def test_a_captured_step_serves_only_the_settings_it_was_captured_with():
+    model = _model("cpu")
+    for change in ("temperature", "top_k", "top_p", "min_p"):
+        s = Sampling(0.9, 10)
+        model._remember_sampling(s)
+        assert model._captured_for(s) and model._captured_for(Sampling(0.9, 10)) and not model._captured_for(None)
+        setattr(s, change, getattr(s, change) / 2 if change != "min_p" else 0.1)      # the same object, with other settings
+        assert not model._captured_for(s)
+    rows = Sampling(torch.tensor([0.9, 1.3]))
+    model._remember_sampling(rows)
+    assert model._captured_for(rows) and model._captured_for(Sampling(rows.temperature))   # (the step reads the tensor anew)
+    assert not model._captured_for(Sampling(rows.temperature.clone()))
+    rows.temperature = torch.tensor([0.9, 1.3])
+    assert not model._captured_for(rows)
+    model._remember_sampling(None)
+    assert model._captured_for(None) and not model._captured_for(Sampling())
+
+
+@pytest.mark.parametrize("top_k", [2.5, 2 ** 31, float("inf"), float("nan")])
+def test_decoder_refuses_a_top_k_that_its_vector_cannot_hold(top_k):
+    prompts, counts = _continuous_case()
+    with pytest.raises(ValueError):
+        ContinuousDecoder(_model("cpu"), 3, sampling=True).run(prompts, counts, sampling=Sampling(1.0, top_k))
+
+
 def test_top_logits_on_cpu():
     model = _model("cpu")
     tokens = torch.randint(0, 64, (2, 21), generator=torch.Generator().manual_seed(2))
@@ -88,6 +113,41 @@ def test_generate_with_a_captured_step_draws_the_eager_tokens():
         assert torch.equal(eager, graphed)
     other, _ = model.generate(prompt, 8, sampling=Sampling(2.0), generator=gen(6))
     assert not torch.equal(other, model.generate(prompt, 8)[0])
+    model.release_graph()
+
+
+@pytest.mark.gpu
+def test_a_captured_step_follows_its_settings():
+    model = _model("cuda")
+    prompt = torch.randint(0, 64, (3, 17), generator=torch.Generator().manual_seed(1)).cuda()
+    gen = lambda: torch.Generator(device="cuda").manual_seed(5)   # noqa: E731
+    s = Sampling(2.0)
+    for temperature in (2.0, 0.0, torch.tensor([0.0, 2.0, 0.0]).cuda(), 1.0):
+        s.temperature = temperature
+        eager, _ = model.generate(prompt, 8, sampling=s, generator=gen())
+        assert torch.equal(eager, model.generate(prompt, 8, use_cuda_graph=True, sampling=s, generator=gen())[0])
+    s.temperature = rows = torch.tensor([0.0, 2.0, 0.0]).cuda()
+    for values in ([0.0, 2.0, 0.0], [2.0, 0.0, 1.0]):             # in place
+        rows.copy_(torch.tensor(values))
+        eager, _ = model.generate(prompt, 8, sampling=s, generator=gen())
+        assert torch.equal(eager, model.generate(prompt, 8, use_cuda_graph=True, sampling=s, generator=gen())[0])
+    model.release_graph()
+
+
+@pytest.mark.gpu
+def test_a_decoder_and_generate_on_one_model():
+    model = _model("cuda")
+    prompts, counts = _continuous_case()
+    prompt = torch.randint(0, 64, (3, 17), generator=torch.Generator().manual_seed(1)).cuda()
+    gen = lambda: torch.Generator(device="cuda").manual_seed(5)   # noqa: E731
+    want = model.generate(prompt, 8)[0]
+    for kw in ({}, dict(sampling=True)):
+        dec = ContinuousDecoder(model, 3, **kw)
+        settings = dict(sampling=Sampling(0.9), generator=gen()) if kw else {}
+        dec.run(prompts, counts, **settings)
+        assert torch.equal(model.generate(prompt, 8, use_cuda_graph=True)[0], want)   # a step of its own: no slots
+        with pytest.raises(RuntimeError):                                             # the decoder's step is gone
+            dec.run(prompts, counts, **settings)
     model.release_graph()
 
 

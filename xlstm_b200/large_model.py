@@ -69,10 +69,8 @@ class Sampling:
     def rows(self, index) -> "Sampling":
         return Sampling(*(v[index] if torch.is_tensor(v) else v for v in (self.temperature, self.top_k, self.top_p, self.min_p)))
 
-    def key(self):
-        """What a captured step depends on; None where the settings lie in tensors (the step reads those anew)."""
-        vals = (self.temperature, self.top_k, self.top_p, self.min_p)
-        return None if any(torch.is_tensor(v) for v in vals) else vals
+    def values(self):
+        return self.temperature, self.top_k, self.top_p, self.min_p
 
 
 def parameter_shapes(cfg: LargeConfig) -> dict:
@@ -531,7 +529,8 @@ class LargeModel:
         for i, st in snapshot.items():   # undo the state changes of the warm-up and capture runs
             for dst, src in zip(self._g_state[i], st):
                 dst.copy_(src)
-        self._graph, self._graph_batch, self._graph_sampling = graph, batch, sampling
+        self._graph, self._graph_batch = graph, batch
+        self._remember_sampling(sampling)
 
     def parameters_on_device(self):
         """Every weight tensor this rank holds (its share under tensor parallelism)."""
@@ -563,7 +562,7 @@ class LargeModel:
         for i in range(max_length):
             if use_cuda_graph and i >= 1:
                 if i == 1:
-                    if getattr(self, "_graph", None) is None or self._graph_batch != B or not self._captured_for(sampling):
+                    if getattr(self, "_graph", None) is None or self._graph_batch != B or self._g_slot is not None or not self._captured_for(sampling):
                         self._capture_decode_graph(state, B, sampling=sampling)
                     else:   # load the fresh prefill state into the graph's static buffers
                         for j, st in state.items():
@@ -583,12 +582,16 @@ class LargeModel:
             ops.check_device_status(self.device)   # synchronises; surfaces a kernel whose bounded wait expired
         return out, state
 
+    def _remember_sampling(self, sampling) -> None:
+        """The settings of the captured step: numbers are part of it, tensors are read anew by every replay (and kept alive here)."""
+        self._graph_sampling = None if sampling is None else sampling.values()
+
     def _captured_for(self, sampling) -> bool:
-        """Whether the captured step draws its tokens as `sampling` says (settings in tensors: only for that very object)."""
+        """Whether the captured step draws its tokens as `sampling` says now: the same numbers, or the very same tensors."""
         had = self._graph_sampling
         if had is None or sampling is None:
             return had is sampling
-        return had is sampling or (had.key() is not None and had.key() == sampling.key())
+        return all(a is b if torch.is_tensor(a) or torch.is_tensor(b) else a == b for a, b in zip(had, sampling.values()))
 
 
 class ContinuousDecoder:
@@ -782,15 +785,17 @@ class ContinuousDecoder:
         start = [0] * len(counts)   # place of a document's first uniform number
         if sampling is not None:
             settings = [sampling] * len(counts) if isinstance(sampling, Sampling) else list(sampling)
-            if len(settings) != len(counts) or any(x.key() is None for x in settings):
+            if len(settings) != len(counts) or any(torch.is_tensor(v) for x in settings for v in x.values()):
                 raise ValueError("one Sampling of numbers per prompt")
             for x in settings:
-                if not (x.temperature >= 0 and x.top_k >= 0 and 0 <= x.top_p <= 1 and 0 <= x.min_p <= 1):
+                if not (x.temperature >= 0 and 0 <= x.top_k < 2 ** 31 and x.top_k == int(x.top_k) and 0 <= x.top_p <= 1 and 0 <= x.min_p <= 1):
                     raise ValueError(f"sampling settings out of range: {x}")
             for d in range(1, len(counts)):
                 start[d] = start[d - 1] + counts[d - 1]
             if counts:
                 self.numbers = self.model._uniform(sum(counts), generator)
+        if self.graphed and self.model._g_tok is not self.tok:
+            raise RuntimeError("the model's captured step is no longer this decoder's (released, or captured anew); make another decoder")
         queue = list(range(len(prompts)))[::-1]
         parked = {}          # document -> parcel of an evicted stream
         left = dict(enumerate(counts))   # document -> tokens still to produce
