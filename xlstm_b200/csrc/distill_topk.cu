@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     }
   }
 
-  bool small = true;   // (this thread's) logits stay below three quarters of the cap
+  bool small = true;   // (this thread's, in the second pass: this warp's) logits stay below three quarters of the cap
   if (LOSS) {
     // both sums over the slice.  The first try takes every magnitude for a small one and looks at the largest behind it;
     // a thread that met a large one sums its vectors again.
@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     __syncwarp();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sR += __shfl_xor_sync(0xffffffffu, sR, o);
+    if (GRAD) small = __all_sync(0xffffffffu, small);   // the second pass's loops meet in whole warps: one way for all lanes
     __syncwarp();
     int all_small = __syncthreads_and(small);   // (and the maximum in s.wf[0] has been read)
     if (lane == 0) s.wf[0][warp] = sR;
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     }
     store(Vec16<T>::round(d), v);
   };
-  if (!live) {
+  if (!live) {   // (`live` is one for the block, `small` for the warp or, from `stats`, for the row: dt_vectors wants whole warps)
     for (int v = slice.v0 + tid; v < slice.v1; v += THREADS) store(make_uint4(0u, 0u, 0u, 0u), v);
   } else if (small) {
     dt_vectors<THREADS>(xv, slice.v0 + tid, slice.v1, [&](const uint4& u, int v) {
