@@ -25,3 +25,29 @@ def test_distill_rows_with_a_few_logits_near_the_cap(tag, rows, tail):
     values, ids, lse = _teacher(g, x[:4], K, 30.0, 1.0, tail, holes=False)
     values, ids, lse = (None if t is None else torch.cat([t, t[-1:].expand(rows - t.shape[0], *t.shape[1:])]) if rows > t.shape[0] else t for t in (values, ids, lse))
     _check_distill(x, values, ids, 30.0, 1.0, lse, torch.rand(rows, generator=g), only=slice(0, 4))
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [501, 70003, 131072])
+def test_sample_rows_without_a_token(tag, V):
+    """Nothing but NaN, nothing but -inf, both: token 0 is drawn, on every way through the row (short ones, and beyond what 16 bits count)."""
+    import xlstm_b200
+    dt = DT[tag]
+    g = torch.Generator().manual_seed(V)
+    x = torch.empty(5, V, dtype=dt)
+    x[0] = math.nan
+    x[1] = -math.inf
+    x[2], x[2, ::2] = math.nan, -math.inf
+    x[3], x[3, :7] = -math.inf, math.nan
+    x[4] = _logits(g, 1, V, dt)[0]
+    u = torch.tensor([0.9, 0.5, 0.999, 0.3, 0.5])
+    for cap in (30.0, None):
+        for kw in ({}, dict(p=0.95, T=0.8), dict(k=300), dict(k=1000, p=0.9, mp=0.01), dict(mp=0.1), dict(k=50), dict(k=1)):
+            got = xlstm_b200.softcap_sample(x.cuda(), cap, u.cuda(), kw.get("T", 1.0), kw.get("k", 0), kw.get("p", 1.0), kw.get("mp", 0.0))
+            assert got[:4].tolist() == [0, 0, 0, 0], kw
+            assert int(got[4]) == O.sample_row(x[4], cap, u[4], **kw)[0]
+        # temperature 0 is the greedy head's token: NaN is passed over, and -inf (under a cap: the value -cap) is a value like any other
+        got = xlstm_b200.softcap_sample(x.cuda(), cap, u.cuda(), 0.0)
+        assert got[:4].tolist() == [0, 0, 0, 7]
+        if cap:
+            assert torch.equal(got, xlstm_b200.softcap_argmax(x.cuda(), cap))

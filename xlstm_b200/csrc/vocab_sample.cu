@@ -72,8 +72,10 @@ struct VsWeights {
   static __device__ __forceinline__ u64 whole(double w) { return vs_whole(w); }
 };
 
-// ceil(sum / each), at most 2^18: the fp32 quotient is off by one at most
+// ceil(sum / each), at most 2^18: the fp32 quotient is off by one at most.  (A place that a mass ends in weighs something; the loop
+// ends without that, too.)
 __device__ __forceinline__ unsigned int vs_steps(u64 sum, u64 each) {
+  if (each == 0ull) return 1u;
   unsigned int q = (unsigned int)((float)sum / (float)each);
   while ((u64)q * each < sum) ++q;
   while (q > 0u && (u64)(q - 1u) * each >= sum) --q;
@@ -761,7 +763,12 @@ template <typename T, int THREADS, int KEEP> __global__ void __launch_bounds__(T
     } else if (!few && !alone) {   // (the digits need the largest logit)
       Selector<T, THREADS, 0> sel(ss, x, p.V, 0, 1);
       sel.bound(1);
-      weigh(float_of_key(ss.top));
+      const float largest = float_of_key(ss.top);
+      if (!(largest > -INFINITY)) {
+        if (threadIdx.x == 0) p.tokens[row] = 0;
+        return;
+      }
+      weigh(largest);
     }
     __syncthreads();
   }

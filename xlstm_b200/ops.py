@@ -366,8 +366,8 @@ def softcap_sample(logits, cap: Optional[float], u, temperature=1.0, top_k=0, to
     the one where the running sum, in order of descending logits, passes ``u`` times the total (``u = 0``: the largest).
 
     A row with temperature 0 takes the token of :func:`softcap_argmax` -- its ties are those of the capped logits rounded to
-    the dtype, where sampling keeps the cap in 64-bit arithmetic.  NaN and -inf logits (masked tokens) are never chosen;
-    a row of nothing else gives token 0."""
+    the dtype, where sampling keeps the cap in 64-bit arithmetic; it passes over NaN only.  NaN and -inf logits (masked
+    tokens) are never drawn; a row of nothing else gives token 0."""
     return native().softcap_sample(logits, cap, u, temperature, top_k, top_p, min_p)
 
 
