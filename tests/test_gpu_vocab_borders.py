@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import vocab as O
-from test_gpu_vocab import DT, _check_distill, _logits, _teacher
+from test_gpu_vocab import DT, _check_distill, _check_sample, _logits, _teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,21 @@ def test_sample_rows_without_a_token(tag, V):
         assert got[:4].tolist() == [0, 0, 0, 7]
         if cap:
             assert torch.equal(got, xlstm_b200.softcap_argmax(x.cuda(), cap))
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [40, 3001, 70003])
+def test_sample_by_numbers_outside_the_unit_interval(tag, V):
+    """u is clamped to [0, 1], NaN counts as 0.  Logits within [-4, 4]: every token weighs more than e^-16, so the last one kept is the
+    same in any arithmetic."""
+    import xlstm_b200
+    g = torch.Generator().manual_seed(V)
+    u = torch.tensor([math.inf, 1e30, 2.0 ** 64, 2.0 ** 21, 2.0, 1.0, math.nan, 0.0, -1e-30, -1.0, -1e30, -math.inf])
+    x = (8 * torch.rand(len(u), V, generator=g) - 4).to(DT[tag])
+    x[1] = 1.0
+    v = u.nan_to_num(0.0, 1.0, 0.0).clamp(0.0, 1.0)
+    for cap, kw in ((30.0, {}), (None, dict(T=0.5, p=0.9)), (30.0, dict(k=7)), (None, dict(k=300, p=0.8)), (30.0, dict(mp=0.3)), (None, dict(k=1)),
+                    (30.0, dict(T=torch.full((len(u),), 0.7), k=torch.arange(len(u), dtype=torch.int32) * 40))):
+        dev = {n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}
+        got = xlstm_b200.softcap_sample(x.cuda(), cap, u.cuda(), dev.get("T", 1.0), dev.get("k", 0), dev.get("p", 1.0), dev.get("mp", 0.0))
+        _check_sample(x, cap, v, got=got, **kw)

@@ -104,8 +104,8 @@ struct VsSettings {
   __device__ __forceinline__ double top_p_goal(u64 kept) const { return ceil((double)top_p * vs_number(kept)); }
   // and the one that u asks for
   __device__ __forceinline__ u64 goal(u64 kept) const {
-    const double at = (double)u * vs_number(kept);
-    return min(kept, at > 0.0 ? (u64)at + 1ull : 1ull);   // (NaN: the first)
+    const double at = (double)(u > 0.f ? fminf(u, 1.f) : 0.f) * vs_number(kept);   // (NaN: the first)
+    return min(kept, (u64)at + 1ull);
   }
 };
 

@@ -363,7 +363,7 @@ def softcap_sample(logits, cap: Optional[float], u, temperature=1.0, top_k=0, to
     order: the weights are ``exp((y - max y) / temperature)`` of the capped logits y; the ``top_k`` largest logits stay (0:
     all; of equal ones the lower indices); of those, a token stays while the tokens in front of it hold less than
     ``top_p`` of their mass; of those, tokens of at least ``min_p`` times the largest weight; always the first.  The token is
-    the one where the running sum, in order of descending logits, passes ``u`` times the total (``u = 0``: the largest).
+    the one where the running sum, in order of descending logits, passes ``u`` times the total (``u = 0``: the largest; from 1 on: the last one kept).
 
     A row with temperature 0 takes the token of :func:`softcap_argmax` -- its ties are those of the capped logits rounded to
     the dtype, where sampling keeps the cap in 64-bit arithmetic; it passes over NaN only.  NaN and -inf logits (masked
