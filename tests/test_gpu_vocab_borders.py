@@ -69,3 +69,22 @@ def test_sample_by_numbers_outside_the_unit_interval(tag, V):
         dev = {n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}
         got = xlstm_b200.softcap_sample(x.cuda(), cap, u.cuda(), dev.get("T", 1.0), dev.get("k", 0), dev.get("p", 1.0), dev.get("mp", 0.0))
         _check_sample(x, cap, v, got=got, **kw)
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [2000, 70003])
+def test_sample_infinite_logits(tag, V):
+    """Under a cap +inf stands at the cap like any other saturated logit; without one the +inf tokens share the row.  On every way."""
+    g = torch.Generator().manual_seed(V + 1)
+    x = _logits(g, 6, V, DT[tag])
+    x[0], x[0, 7] = 25.0, math.inf                       # y = 20.5 for all but one of 30
+    x[1, 11], x[1, 500], x[1, 900] = math.inf, 500.0, 40.0
+    x[2, ::2], x[2, 3] = 1000.0, math.inf                # half of the row saturated
+    x[3, 5:] = -math.inf
+    x[3, :5] = torch.tensor([math.inf, 500.0, 0.0, 29.0, math.inf])
+    x[4, ::3], x[4, 1] = math.nan, math.inf
+    x[5, 100], x[5, 200] = math.inf, -math.inf
+    u = torch.tensor([0.9, 0.6, 0.77, 0.9, 0.9999, 0.99995])
+    for cap, kw in ((30.0, {}), (30.0, dict(T=8.0)), (30.0, dict(T=3.0, p=0.99)), (30.0, dict(k=40, T=20.0)), (30.0, dict(k=400, T=10.0)), (30.0, dict(mp=0.05, T=4.0)), (1.0, dict(T=0.3)),
+                    (None, {}), (None, dict(k=40)), (None, dict(p=0.5)), (None, dict(mp=0.1))):
+        _check_sample(x, cap, u, **kw)

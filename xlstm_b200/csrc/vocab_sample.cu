@@ -57,7 +57,7 @@ struct VsWeights {
   __device__ __forceinline__ void set_max() { ymax = capped(largest); }
   __device__ __forceinline__ double of(float v, double y) const {
     const double w = exp64((y - ymax) * invT);
-    return v == largest ? 1.0 : !(v > -INFINITY) || largest == INFINITY ? 0.0 : w;   // 0: NaN and -inf; next to +inf
+    return v == largest ? 1.0 : !(v > -INFINITY) || (largest == INFINITY && !(cap > 0.0)) ? 0.0 : w;   // 0: NaN and -inf; next to +inf without a cap
   }
   __device__ __forceinline__ double of(float v) const { return of(v, capped(v)); }
   // several at a time, the largest's cap among them: a 64-bit instruction's result takes some forty cycles
