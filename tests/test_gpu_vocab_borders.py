@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import vocab as O
-from test_gpu_vocab import DT, _check_distill, _check_sample, _logits, _teacher
+from test_gpu_vocab import DT, E24, _check_distill, _check_sample, _logits, _rel, _teacher
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,28 @@ def test_sample_infinite_logits(tag, V):
     for cap, kw in ((30.0, {}), (30.0, dict(T=8.0)), (30.0, dict(T=3.0, p=0.99)), (30.0, dict(k=40, T=20.0)), (30.0, dict(k=400, T=10.0)), (30.0, dict(mp=0.05, T=4.0)), (1.0, dict(T=0.3)),
                     (None, {}), (None, dict(k=40)), (None, dict(p=0.5)), (None, dict(mp=0.1))):
         _check_sample(x, cap, u, **kw)
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [300, 20011])
+def test_topk_sums_of_rows_with_nan_and_infinities(tag, V):
+    """A NaN anywhere makes the log-sum-exp NaN, also in a row without a number or with +inf; without one it is -inf, +inf or a number."""
+    import xlstm_b200
+    dt = DT[tag]
+    g = torch.Generator().manual_seed(V)
+    x = _logits(g, 7, V, dt)
+    x[0] = math.nan
+    x[1], x[1, 5] = -math.inf, math.nan
+    x[2, 8], x[2, 9] = math.inf, math.nan
+    x[3] = -math.inf
+    x[4, 3] = math.inf
+    x[5], x[5, 250] = math.nan, 1.0
+    x[6, 2] = -math.inf
+    for cap, T in ((None, 1.0), (None, 0.1), (30.0, 1.0), (30.0, 0.1)):
+        values, ids, lse = xlstm_b200.softcap_topk(x.cuda(), cap, 3, T)
+        for r in range(7):
+            y, idx, l = O.topk_row(x[r], cap, 3, T)
+            assert ids[r].tolist() == idx
+            torch.testing.assert_close(values[r].cpu().double(), y, rtol=8 * E24, atol=0, equal_nan=True)
+            zmax = float((y[torch.isfinite(y)].abs() / T).max()) if bool(torch.isfinite(y).any()) else 0.0   # (the terms that count)
+            torch.testing.assert_close(lse[r].cpu().double(), l, rtol=E24, atol=_rel(zmax) + 64 * E24, equal_nan=True)

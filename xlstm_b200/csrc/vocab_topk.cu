@@ -74,7 +74,7 @@ template <typename T, bool CAP, bool BOUNDED, int THREADS, int KEEP> __global__ 
       sum = s.from[0];
       for (int r = 1; r < blocks; ++r) sum += s.from[r];
     }
-    p.lse[row] = isinf(largest) && !CAP ? largest : (float)((log2_64((double)sum) + (double)zmax) * 0.69314718055994530942 + (CAP ? 0.0 : (double)Z.ref * invT));
+    p.lse[row] = (float)((log2_64((double)sum) + (double)zmax) * 0.69314718055994530942 + (CAP ? 0.0 : (double)Z.ref * invT));
   }
   if (n > SEL_CAP || n < (unsigned int)k) {
     select_exact<T, THREADS>(s.exact, s.sel.list, x, p.V, k);
