@@ -457,7 +457,8 @@ template <typename T, bool CAP, bool BOUNDED, bool LOSS, bool GRAD> static int d
   const int blocks = dt_blocks(p->rows, p->V);
   auto kern = distill_kernel<T, CAP, BOUNDED, LOSS, GRAD>;
   const size_t smem = dt_smem(p->K, p->V, Vec16<T>::N, blocks);
-  if (smem > 40 * 1024) XL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  // (one limit for all calls: the attribute is the kernel's, and another host thread may set it between here and the launch)
+  if (smem > 40 * 1024) XL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dt_smem(TOPK_MAX, VOCAB_MAX, Vec16<T>::N, 1)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p->rows * blocks);
   cfg.blockDim = dim3(dt_threads(LOSS && GRAD));
