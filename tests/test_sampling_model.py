@@ -221,3 +221,30 @@ def test_a_teacher_and_a_student_and_its_tokens(dtype):
     drawn = xlstm_b200.softcap_sample(logits.detach(), 30.0, torch.rand(B, S, generator=g).cuda(), 0.8, 10, 0.9)
     kept = xlstm_b200.softcap_topk(logits.detach(), 30.0, 10)[1]
     assert bool((kept == drawn[..., None]).any(-1).all())    # every token is one of its row's ten largest
+
+
+def test_sampling_off_the_gpu_is_the_operators_definition():
+    """Masked, NaN and infinite logits, numbers outside [0, 1), settings per row: large_model._sample against the oracle."""
+    import math
+
+    from xlstm_b200 import large_model as L
+    g = torch.Generator().manual_seed(12)
+    x = 3 * torch.randn(11, 200, generator=g)
+    x[0, ::2] = math.nan
+    x[1, 5:] = -math.inf
+    x[2] = math.nan
+    x[3] = -math.inf
+    x[4], x[4, ::3] = -math.inf, math.nan
+    x[5, 7], x[5, 8], x[5, 9:40] = math.inf, math.nan, 500.0
+    x[6, 100] = math.inf
+    x[7, 199] = math.nan
+    x[8] = 2.0
+    u = torch.tensor([0.3, 0.9, 0.9, 0.9, 0.9, 0.9, 0.5, 0.999, 2.0, math.nan, -1.0])
+    for kw in ({}, dict(T=0.5, k=20), dict(T=4.0, p=0.8), dict(mp=0.2), dict(T=3.0, k=150, p=0.9, mp=0.01)):
+        s = Sampling(kw.get("T", 1.0), kw.get("k", 0), kw.get("p", 1.0), kw.get("mp", 0.0))
+        got = L._sample(x, 30.0, u, s)
+        assert got.shape == (11, 1)
+        for r in range(11):
+            assert int(got[r]) == V.sample_row(x[r], 30.0, u[r].nan_to_num(0.0), **kw)[0], (kw, r)
+    greedy = L._sample(x, 30.0, u, Sampling(0.0))[:, 0]          # NaN is passed over, -inf stands at -cap
+    assert greedy.tolist() == [int(torch.argmax((30.0 * torch.tanh(r / 30.0)).nan_to_num(-math.inf))) for r in x]

@@ -123,16 +123,17 @@ def _sample(logits, cap, u, s: Sampling):
     n = logits.shape[0]
     T, k, p, mp = (torch.as_tensor(v, device=logits.device).expand(n)[:, None] for v in (s.temperature, s.top_k, s.top_p, s.min_p))
     T, p, mp = T.float().double(), p.float().double(), mp.float().double()
-    x, idx = torch.sort(logits.double(), dim=-1, descending=True, stable=True)
+    nan = torch.isnan(logits)   # never drawn, like -inf
+    x, idx = torch.sort(logits.double().masked_fill(nan, -math.inf), dim=-1, descending=True, stable=True)
     y = _soft_cap(x, cap)
     w = torch.exp((y - y[:, :1]) / T.clamp(min=1e-30))
-    w = torch.where((torch.arange(x.shape[1], device=x.device) < k) | (k <= 0), w, 0.0)
+    w = torch.where(((torch.arange(x.shape[1], device=x.device) < k) | (k <= 0)) & (x > -math.inf), w, 0.0)
     upto = torch.cumsum(w, -1)
     keep = (((upto - w) < p * upto[:, -1:]) | (p >= 1)) & (w >= mp) & (w > 0)
     keep[:, 0] = True
     at = (upto <= u.double()[:, None] * torch.where(keep, w, 0.0).sum(-1, keepdim=True)).sum(-1)
     drawn = idx.gather(1, torch.minimum(at, keep.sum(-1) - 1)[:, None])
-    return torch.where(T > 0, drawn, torch.argmax(_soft_cap(logits, cap), dim=-1, keepdim=True))
+    return torch.where(T > 0, drawn, torch.argmax(_soft_cap(logits, cap).masked_fill(nan, -math.inf), dim=-1, keepdim=True))
 
 
 def _top(logits, cap, k: int, temperature: float):
