@@ -248,3 +248,24 @@ def test_sampling_off_the_gpu_is_the_operators_definition():
             assert int(got[r]) == V.sample_row(x[r], 30.0, u[r].nan_to_num(0.0), **kw)[0], (kw, r)
     greedy = L._sample(x, 30.0, u, Sampling(0.0))[:, 0]          # NaN is passed over, -inf stands at -cap
     assert greedy.tolist() == [int(torch.argmax((30.0 * torch.tanh(r / 30.0)).nan_to_num(-math.inf))) for r in x]
+
+
+def test_top_logits_off_the_gpu_are_the_operators_definition():
+    """NaN comes last, behind -inf; equal logits by index."""
+    import math
+
+    from xlstm_b200 import large_model as L
+    g = torch.Generator().manual_seed(13)
+    x = torch.randint(-3, 4, (6, 40), generator=g).float()
+    x[0, ::2] = math.nan
+    x[1], x[1, ::3] = -math.inf, math.nan
+    x[2] = math.nan
+    x[3, 5], x[3, 6], x[3, 7] = math.inf, -math.inf, math.nan
+    x[4] = -math.inf
+    for k in (1, 7, 40):
+        values, ids, lse = L._top(x, 30.0, k, 2.0)
+        for r in range(6):
+            y, idx, l = V.topk_row(x[r], 30.0, k, 2.0)
+            assert ids[r].tolist() == idx
+            torch.testing.assert_close(values[r].double(), y, rtol=1e-6, atol=0, equal_nan=True)
+            torch.testing.assert_close(lse[r].double(), l, rtol=1e-6, atol=1e-6, equal_nan=True)

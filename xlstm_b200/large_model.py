@@ -139,7 +139,9 @@ def _sample(logits, cap, u, s: Sampling):
 def _top(logits, cap, k: int, temperature: float):
     """``ops.softcap_topk`` on any device."""
     y = _soft_cap(logits.float(), cap)
-    ids = torch.sort(logits, dim=-1, descending=True, stable=True).indices[..., :k]
+    nan = torch.isnan(logits)   # behind everything else
+    ids = torch.sort(logits.masked_fill(nan, -math.inf), dim=-1, descending=True, stable=True).indices
+    ids = ids.gather(-1, torch.sort(nan.gather(-1, ids).to(torch.uint8), dim=-1, stable=True).indices)[..., :k]
     return y.gather(-1, ids), ids.to(torch.int32), torch.logsumexp(y / temperature, -1)
 
 
