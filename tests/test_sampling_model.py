@@ -269,3 +269,25 @@ def test_top_logits_off_the_gpu_are_the_operators_definition():
             assert ids[r].tolist() == idx
             torch.testing.assert_close(values[r].double(), y, rtol=1e-6, atol=0, equal_nan=True)
             torch.testing.assert_close(lse[r].double(), l, rtol=1e-6, atol=1e-6, equal_nan=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S", [1, 5])
+def test_top_logits_leave_the_callers_state_as_it_was(dtype, S):
+    """The states are not handed back, so the given ones stay those in front of the tokens (a decode step updates C in place)."""
+    model = LargeModel(CFG, procedural_state_dict(CFG, 4), "cuda", dtype)
+    g = torch.Generator().manual_seed(1)
+    prompt, more = (torch.randint(0, 64, (3, n), generator=g).cuda() for n in (17, S))
+    _, state = model.forward(prompt)
+    before = {i: tuple(t.clone() for t in st) for i, st in state.items()}
+    first = model.top_logits(more, 5, 1.0, state=state)
+    for i, st in state.items():
+        assert all(torch.equal(a, b) for a, b in zip(st, before[i]))
+    again = model.top_logits(more, 5, 1.0, state=state)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    logits, _ = model.forward(more, state)
+    # cap * tanh(x / cap): three roundings by half a step on either side (tanh in fp32 by two steps: 8 half steps in all, twice); in
+    # bf16 on the side of the logits alone
+    tol = 16 * 2.0 ** -24 if dtype is torch.float32 else 3.1 * 2.0 ** -8
+    torch.testing.assert_close(first[0], logits.float().topk(5, dim=-1).values, rtol=tol, atol=0)

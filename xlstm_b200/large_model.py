@@ -480,7 +480,10 @@ class LargeModel:
     @torch.no_grad()
     def top_logits(self, tokens, k: int, temperature: float = 1.0, state=None, cu_seqlens=None):
         """A teacher's view of `tokens` (B,S): ``values, ids, lse`` of :func:`ops.softcap_topk` for every position, (B,S,k),
-        (B,S,k) and (B,S) -- what ``ops.distill_topk`` takes.  The logits of more than 4096 positions are never held at once."""
+        (B,S,k) and (B,S) -- what ``ops.distill_topk`` takes.  The logits of more than 4096 positions are never held at once.
+        A given ``state`` stays as it is."""
+        if state is not None and tokens.shape[1] == 1 and cu_seqlens is None:   # (a decode step updates C in place)
+            state = {i: (c.clone(), n, m) for i, (c, n, m) in state.items()}
         return self.forward(tokens, state, cu_seqlens=cu_seqlens, top=(k, temperature))[0]
 
     def _uniform(self, n: int, generator=None):
