@@ -291,3 +291,47 @@ def test_top_logits_leave_the_callers_state_as_it_was(dtype, S):
     # bf16 on the side of the logits alone
     tol = 16 * 2.0 ** -24 if dtype is torch.float32 else 3.1 * 2.0 ** -8
     torch.testing.assert_close(first[0], logits.float().topk(5, dim=-1).values, rtol=tol, atol=0)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_drawing_does_not_depend_on_the_default_type(default):
+    """Uniform numbers, the slots' settings and the captured step's buffers are float32 whatever torch's default is."""
+    model = _model("cpu")
+    prompt = torch.randint(0, 64, (3, 17), generator=torch.Generator().manual_seed(1))
+    prompts, counts = _continuous_case()
+    gen = lambda: torch.Generator().manual_seed(5)   # noqa: E731
+    s = Sampling(0.9, 12, 0.95, 0.01)
+
+    def draw():
+        return [model._uniform(100, gen()), model.generate(prompt, 6, sampling=s, generator=gen())[0],
+                *ContinuousDecoder(model, 3, sampling=True).run(prompts, counts, sampling=s, generator=gen())]
+    want = draw()
+    torch.set_default_dtype(default)
+    try:
+        got = draw()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert got[0].dtype == torch.float32
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_captured_draws_do_not_depend_on_the_default_type():
+    model = _model("cuda")
+    prompt = torch.randint(0, 64, (3, 17), generator=torch.Generator().manual_seed(1)).cuda()
+    prompts, counts = _continuous_case()
+    gen = lambda: torch.Generator(device="cuda").manual_seed(5)   # noqa: E731
+    s = Sampling(0.9, 12, 0.95, 0.01)
+
+    def draw():
+        out = [model.generate(prompt, 6, use_cuda_graph=True, sampling=s, generator=gen())[0].cpu(),
+               *ContinuousDecoder(model, 3, sampling=True).run(prompts, counts, sampling=s, generator=gen())]
+        model.release_graph()
+        return out
+    want = draw()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = draw()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -121,8 +121,8 @@ def _soft_cap(x, cap):
 def _sample(logits, cap, u, s: Sampling):
     """``ops.softcap_sample`` on any device, in 64-bit torch operations (the kernel is what runs on CUDA)."""
     n = logits.shape[0]
-    T, k, p, mp = (torch.as_tensor(v, device=logits.device).expand(n)[:, None] for v in (s.temperature, s.top_k, s.top_p, s.min_p))
-    T, p, mp = T.float().double(), p.float().double(), mp.float().double()
+    T, p, mp = (torch.as_tensor(v, dtype=torch.float32, device=logits.device).double().expand(n)[:, None] for v in (s.temperature, s.top_p, s.min_p))
+    k = torch.as_tensor(s.top_k, device=logits.device).expand(n)[:, None]
     nan = torch.isnan(logits)   # never drawn, like -inf
     x, idx = torch.sort(logits.double().masked_fill(nan, -math.inf), dim=-1, descending=True, stable=True)
     y = _soft_cap(x, cap)
@@ -488,7 +488,7 @@ class LargeModel:
 
     def _uniform(self, n: int, generator=None):
         """n uniform numbers in [0, 1) on the model's device; with tensor parallelism the same on all ranks."""
-        u = torch.rand(n, device=self.device, generator=generator)
+        u = torch.rand(n, dtype=torch.float32, device=self.device, generator=generator)
         if self.tp_world > 1:
             torch.distributed.broadcast(u, 0 if self.group is None else torch.distributed.get_global_rank(self.group, 0), group=self.group)
         return u
@@ -507,7 +507,7 @@ class LargeModel:
         self._g_tok = torch.zeros(batch, 1, dtype=torch.long, device=dev)
 
         self._g_slot = slot_map
-        self._g_u = torch.zeros(batch, device=dev)
+        self._g_u = torch.zeros(batch, dtype=torch.float32, device=dev)
 
         def body():
             nxt, st = self.forward(self._g_tok, self._g_state, greedy=True, slot=self._g_slot, sampling=sampling, u=self._g_u)
@@ -629,20 +629,21 @@ class ContinuousDecoder:
         self.graphed = (dev.type == "cuda") if use_cuda_graph is None else use_cuda_graph
         self.packed = (dev.type == "cuda" and model.cell is ops) if packed_admission is None else packed_admission
         self.row_len, self.max_rows = row_len, max_rows_per_prefill
-        self.state = {i: (torch.zeros(num_slots, model.nh_local, model.dq, model.dv, device=dev),
-                          torch.zeros(num_slots, model.nh_local, model.dq, device=dev),
-                          torch.zeros(num_slots, model.nh_local, 1, device=dev)) for i in range(cfg.num_blocks)}
+        f32 = dict(dtype=torch.float32, device=dev)
+        self.state = {i: (torch.zeros(num_slots, model.nh_local, model.dq, model.dv, **f32),
+                          torch.zeros(num_slots, model.nh_local, model.dq, **f32),
+                          torch.zeros(num_slots, model.nh_local, 1, **f32)) for i in range(cfg.num_blocks)}
         self.tok = torch.zeros(num_slots, 1, dtype=torch.long, device=dev)
         self.slots = SlotPool(num_slots)
         self.slot_map = torch.full((num_slots,), -1, dtype=torch.int32, device=dev) if dev.type == "cuda" and model.cell is ops else None
         self.prefill_calls = 0
         self.sampling = None
         if sampling:
-            self.sampling = Sampling(torch.zeros(num_slots, device=dev), torch.zeros(num_slots, dtype=torch.int32, device=dev),
-                                     torch.ones(num_slots, device=dev), torch.zeros(num_slots, device=dev))
-            self.u = torch.zeros(num_slots, device=dev)
+            self.sampling = Sampling(torch.zeros(num_slots, **f32), torch.zeros(num_slots, dtype=torch.int32, device=dev),
+                                     torch.ones(num_slots, **f32), torch.zeros(num_slots, **f32))
+            self.u = torch.zeros(num_slots, **f32)
             self.cursor = torch.zeros(num_slots, dtype=torch.long, device=dev)   # place of the slot's next number in `numbers`
-            self.numbers = torch.zeros(1, device=dev)
+            self.numbers = torch.zeros(1, **f32)
         if self.graphed:
             if self.slot_map is not None:
                 self.slot_map.copy_(torch.arange(num_slots, dtype=torch.int32, device=dev))   # capture with every row live
