@@ -453,7 +453,8 @@ int xl_softcap_argmax_noalloc(const xl_greedy_params* p, void* cuda_stream);
  * the first token always stays.  The result is the first token whose running sum of kept w exceeds u times their total.
  * A row with temperature <= 0 or NaN takes the token of xl_softcap_argmax, which passes over NaN only (under a cap -inf is -cap;
  * a row of NaN gives token 0).  No draw takes NaN or -inf (a row of nothing else gives token 0); with a +inf logit and no cap
- * the +inf tokens share the row.  u outside [0, 1) is clamped (NaN: 0).
+ * the +inf tokens share the row.  u outside [0, 1) is clamped (NaN: 0).  Sums are kept in units of 2^-44: a token of w < 2^-45 has no
+ * part in them.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct xl_sample_params {
   const void* logits;       /* (rows, V) un-capped logits, dtype `dtype`, row stride row_stride elements */

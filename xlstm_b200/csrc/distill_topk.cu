@@ -9,10 +9,14 @@
 // 1e-9 behind a confident student nor the named tokens behind a flat one come out of a difference of large numbers, and
 // the tail's factor W e^{l_R - l} - p_t is one number a row.  The K teacher entries are few: their terms are in 64 bits.
 //
-// What bounds it.  The fp32 pipe and the exponentials: 10 instructions a logit for the loss (2048 rows of 50 304 in bf16: 57 us, their
-// 206 MB are 31 us of memory), the gradient alone 79 us (413 MB, 63 us), both in one launch 24 instructions (4096 rows: 241 us; the logits come
-// from memory once, 826 MB in all, 126 us).  Few rows: the chain ids -> logits there -> 64-bit exponentials -> sums -> logarithms -> gradient,
-// 12 us for 64 rows cut over clusters of eight blocks.
+// What bounds it.  Waiting, with the fp32 units half and those of the special functions two fifths busy and 2.1 instructions a cycle and
+// SM of 4: per instruction a warp waits 3 cycles for loads in the loss (11 instructions a logit; 2048 rows of 50 304 in bf16: 58 us, their
+// 206 MB are 31 us of memory), 10 in the gradient alone (10 instructions; 77 us, 413 MB, 63 us), 5 and 2.4 at barriers with both in
+// one launch (22 instructions; 4096 rows: 236 us; the logits come from memory once, 826 MB in all, 126 us).  Few rows: the chain ids ->
+// logits there -> 64-bit exponentials -> sums -> logarithms -> gradient, 12 us for 64 rows cut over clusters of eight blocks.
+// These are rows whose logits stay below three quarters of the cap.  One beyond it sends its thread over its vectors again, with a
+// branch and a division an element, and in the backward launch the whole row: one such logit a row 111 us for the loss, 230 for
+// loss and gradient through autograd (135 without), 368 for 4096 rows in one launch (64 of them a row: 139, 259, 427).
 #include "vocab_row.cuh"
 
 namespace xl {

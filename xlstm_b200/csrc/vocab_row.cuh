@@ -118,8 +118,9 @@ __device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// tanh(z) = z P(z^2) for |z| <= 0.75, relative error within 3 * 2^-24 (least-squares weights driven to the minimax, degree 5);
-// a model's logits stay below three quarters of the cap.  Beyond it 1 - 2 / (1 + e^2|z|), whose quotient is below 0.37 there.
+// tanh(z) = z P(z^2) for |z| <= 0.75, relative error within 3 * 2^-24 (least-squares weights driven to the minimax, degree 5).
+// Rows whose logits all stay below three quarters of the cap are fast; what larger ones cost stands at the kernels.
+// Beyond it 1 - 2 / (1 + e^2|z|), whose quotient is below 0.37 there.
 constexpr float TANH_SMALL = 0.75f;
 __device__ __forceinline__ float tanh_large(float z) {
   const float q = 1.f - __fdividef(2.f, 1.f + exp2_approx(fminf(fabsf(z), 20.f) * (2.f * LOG2E)));

@@ -4,9 +4,12 @@
 // of groups for a bound of the k-th largest (vocab_select.cuh), then the list of what reaches it together with the sum of
 // 2^(z - z_max) in fp32.  The second pass finds the row in L2, so memory is read once.
 //
-// What bounds it.  Many rows: issue slots and load latency, 16 instructions a logit in both passes (of which the cap's polynomial,
-// exponential and sum are 7.5) at 2.2 instructions a cycle and SM: 4096 rows of 50 304 in bf16, k = 64, take 143 us, where their 412 MB are
-// 63 us of memory.  Few rows: the chain of maxima, bisection, list and sort, 8.5 us for 16 rows, cut over clusters of eight blocks.
+// What bounds it.  Many rows: waiting; no unit is full.  15 instructions a logit in both passes (of which the cap's polynomial,
+// exponential and sum are 7.5) at 2.1 a cycle and SM of 4; per instruction a warp waits 3.3 cycles for loads and 2.4 at barriers, the fp32
+// units are busy 37 % of the time, those of the special functions 34 %.  4096 rows of 50 304 in bf16, k = 64, take 144 us, where their
+// 412 MB are 63 us of memory (k = 256: 217 us; from k of some 440 on the list overflows and the exact selection does all: k = 512, 1.5 ms).
+// A logit beyond three quarters of the cap sends its thread over its vectors again: one a row 211 us, 64 a row 266.
+// Few rows: the chain of maxima, bisection, list and sort, 8.2 - 8.9 us for 16 rows, cut over clusters of eight blocks.
 #include "vocab_select.cuh"
 
 namespace xl {
