@@ -113,3 +113,17 @@ def test_topk_sums_of_rows_with_nan_and_infinities(tag, V):
             torch.testing.assert_close(values[r].cpu().double(), y, rtol=8 * E24, atol=0, equal_nan=True)
             zmax = float((y[torch.isfinite(y)].abs() / T).max()) if bool(torch.isfinite(y).any()) else 0.0   # (the terms that count)
             torch.testing.assert_close(lse[r].cpu().double(), l, rtol=E24, atol=_rel(zmax) + 64 * E24, equal_nan=True)
+
+
+def test_rows_beyond_32_bits_are_refused():
+    """A row length is not cut to 32 bits on its way to the kernel (2^32 + 8 tokens are not 8)."""
+    import xlstm_b200
+    from xlstm_b200._lib import XlError
+    values, ids = torch.zeros(1, 3).cuda(), torch.zeros(1, 3, dtype=torch.int32).cuda()
+    for V in (2 ** 31, 2 ** 32 + 8):
+        x = torch.zeros(1, V, dtype=torch.bfloat16, device="cuda")
+        for call in (lambda: xlstm_b200.softcap_sample(x, 30.0, torch.zeros(1).cuda()), lambda: xlstm_b200.softcap_topk(x, None, 3),
+                     lambda: xlstm_b200.distill_topk(x, values, ids), lambda: xlstm_b200.distill_topk_grad(x, values, ids)):
+            with pytest.raises(XlError, match="capacity"):
+                call()
+        del x

@@ -763,6 +763,7 @@ struct VocabRows {
     TORCH_CHECK_VALUE(rows <= INT32_MAX, name, ": too many rows");
   }
   int64_t stride() const { return rows > 1 ? x.stride(0) : V; }
+  int32_t length() const { return (int32_t)std::min<int64_t>(V, INT32_MAX); }   // (far too long either way: the entry says so)
   // one value per row: any shape of that many elements
   Tensor per_row(const Tensor& t, const char* name, const char* what) const {
     TORCH_CHECK_VALUE(t.device() == x.device() && t.numel() == rows, name, ": ", what, " must have one entry per row of logits, on their device");
@@ -822,7 +823,7 @@ PyObject* softcap_sample(PyObject*, PyObject* const* a, Py_ssize_t na) {
   int rc = XL_OK;
   if (r.rows > 0) {
     p.logits = r.x.data_ptr(); p.tokens = out.data_ptr<int64_t>(); p.u = u.const_data_ptr<float>();
-    p.rows = (int32_t)r.rows; p.V = (int32_t)r.V; p.row_stride = r.stride(); p.cap = r.cap;
+    p.rows = (int32_t)r.rows; p.V = r.length(); p.row_stride = r.stride(); p.cap = r.cap;
     p.temperature = (float)temperature.value; p.top_k = (int32_t)top_k.value; p.top_p = (float)top_p.value; p.min_p = (float)min_p.value;
     p.dtype = dtype_code(r.x);
     rc = xl_softcap_sample(&p, stream_of(r.x));
@@ -854,7 +855,7 @@ PyObject* softcap_topk(PyObject*, PyObject* const* a, Py_ssize_t na) {
   if (r.rows > 0) {
     xl_topk_params p = {};
     p.logits = r.x.data_ptr(); p.values = values.data_ptr<float>(); p.ids = ids.data_ptr<int32_t>(); p.lse = lse.data_ptr<float>();
-    p.rows = (int32_t)r.rows; p.V = (int32_t)r.V; p.k = (int32_t)std::min<int64_t>(k, INT32_MAX); p.row_stride = r.stride(); p.cap = r.cap;
+    p.rows = (int32_t)r.rows; p.V = r.length(); p.k = (int32_t)std::min<int64_t>(k, INT32_MAX); p.row_stride = r.stride(); p.cap = r.cap;
     p.temperature = (float)temperature; p.dtype = dtype_code(r.x);
     rc = xl_softcap_topk(&p, stream_of(r.x));
   }
@@ -896,7 +897,7 @@ struct DistillArgs {
       p.weight = weight.const_data_ptr<float>();
       p.weight_stride = one ? 0 : weight.stride(0);
     }
-    p.rows = (int32_t)r.rows; p.V = (int32_t)r.V; p.K = (int32_t)std::min<int64_t>(K, INT32_MAX);
+    p.rows = (int32_t)r.rows; p.V = r.length(); p.K = (int32_t)std::min<int64_t>(K, INT32_MAX);
     p.row_stride = r.stride(); p.dlogits_stride = r.V;
     p.cap = r.cap; p.temperature = (float)temperature; p.dtype = dtype_code(r.x);
   }

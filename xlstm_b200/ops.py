@@ -357,7 +357,7 @@ def softcap_argmax(logits, cap: float):
 def softcap_sample(logits, cap: Optional[float], u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Sampled tokens of un-capped logits, from given uniform numbers: int64 of shape ``logits.shape[:-1]``.
 
-    ``logits`` (..., V), ``cap`` the soft cap of the model's logits (None: none), ``u`` one float32 number in [0, 1) per
+    ``logits`` (..., V), V up to 2**18, ``cap`` the soft cap of the model's logits (None: none), ``u`` one float32 number in [0, 1) per
     row.  ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are numbers, or CUDA tensors of one per row (numbers are
     checked, tensors are not looked at: values outside their range act like the end of it).  They are applied in that
     order: the weights are ``exp((y - max y) / temperature)`` of the capped logits y; the ``top_k`` largest logits stay (0:
@@ -375,7 +375,7 @@ def softcap_topk(logits, cap: Optional[float], k: int, temperature: float = 1.0)
     """The ``k`` largest soft-capped logits of every row and the row's log-sum-exp: what a teacher leaves for
     :func:`distill_topk`.  Returns ``values`` (..., k) float32 (capped, not divided by the temperature, descending; equal
     logits: lower index first; NaN last), ``ids`` (..., k) int32 and ``lse`` (...) float32, the log of the sum of
-    ``exp(y / temperature)`` over all V.  ``k`` up to 1024.  Not recorded by autograd."""
+    ``exp(y / temperature)`` over all V.  ``k`` up to 1024, V up to 2**18.  Not recorded by autograd."""
     return native().softcap_topk(logits, cap, k, temperature)
 
 
@@ -399,7 +399,7 @@ class DistillFunction(torch.autograd.Function):
 def distill_topk(logits, values, ids, cap: Optional[float] = None, temperature: float = 1.0, teacher_lse=None):
     """Distillation loss of every row against a teacher's top logits, differentiable in ``logits``.
 
-    ``logits`` (..., V) un-capped, of the student; ``values`` and ``ids`` (..., K) as :func:`softcap_topk` gives them (an id
+    ``logits`` (..., V) un-capped, of the student, V up to 2**18; ``values`` and ``ids`` (..., K) as :func:`softcap_topk` gives them (an id
     below 0: unused entry; K up to 1024).  With T the temperature, q the softmax of the student's capped logits over T and p
     the softmax of the entries over T, the loss is ``T**2 * sum p (log p - log q)`` (float32, shape ``logits.shape[:-1]``).
     With ``teacher_lse`` -- the teacher's log-sum-exp over its whole vocabulary at the same temperature -- p are the
