@@ -42,7 +42,7 @@ typedef enum xl_status {
   XL_ERR_NULL_POINTER = -1,
   XL_ERR_BAD_SHAPE = -2,       /* a dimension is zero/negative or not supported by the kernel */
   XL_ERR_BAD_STRIDE = -3,      /* stride not compatible with 16-byte vector / TMA access */
-  XL_ERR_BAD_ALIGNMENT = -4,   /* base pointer not 16-byte aligned */
+  XL_ERR_BAD_ALIGNMENT = -4,   /* base pointer not 16-byte aligned (or as the entry says) */
   XL_ERR_BAD_DTYPE = -5,
   XL_ERR_UNSUPPORTED = -6,     /* valid request, but not by this entry point (use the one named in the docs) */
   XL_ERR_CUDA = -7,            /* a CUDA runtime/driver call failed; see xl_last_cuda_error() */
@@ -469,7 +469,8 @@ typedef struct xl_sample_params {
   int32_t dtype;
 } xl_sample_params;
 
-/* Requires V <= 2^18.  Needs no scratch memory; calls may overlap. */
+/* Requires V <= 2^18 and logits at a multiple of the element's size (here and in the entries below; any such address and
+ * row stride).  Needs no scratch memory; calls may overlap. */
 int xl_softcap_sample(const xl_sample_params* p, void* cuda_stream);
 
 /* ------------------------------------------------------------------------------------------------

@@ -79,3 +79,21 @@ def test_operators_refuse_host_tensors():
         xlstm_b200.softcap_sample(x, 30.0, u, temperature=-1.0)
     with pytest.raises(ValueError, match="cap"):
         xlstm_b200.softcap_topk(x, 0.0, 2)
+
+
+def test_entries_refuse_addresses_inside_an_element():
+    from xlstm_b200 import _lib
+    l = _lib.lib()
+    for dtype, off in ((0, 1), (0, 2), (1, 1)):
+        s, t, d = _lib.SampleParams(), _lib.TopkParams(), _lib.DistillParams()
+        for p in (s, t, d):
+            p.logits, p.rows, p.V, p.row_stride, p.dtype, p.temperature = 0x1000 + off, 2, 8, 8, dtype, 1.0
+        s.tokens = s.u = 0x2000
+        t.values = t.ids = d.values = d.ids = d.loss = 0x2000
+        t.k = d.K = 2
+        assert l.xl_softcap_sample(ctypes.byref(s), None) == -4
+        assert l.xl_softcap_topk(ctypes.byref(t), None) == -4
+        assert l.xl_distill_topk(ctypes.byref(d), None) == -4
+        d.logits, d.dlogits, d.dlogits_stride, d.stats = 0x1000, 0x8000 + off, 8, 0x9000
+        for entry in (l.xl_distill_topk, l.xl_distill_topk_backward):
+            assert entry(ctypes.byref(d), None) == -4

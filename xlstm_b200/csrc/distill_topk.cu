@@ -435,11 +435,11 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
 
 static int dt_validate(const xl_distill_params* p) {
   if (!p || !p->logits || !p->values || !p->ids) return XL_ERR_NULL_POINTER;
-  const int rc = vocab_validate(p->rows, p->V, p->row_stride, p->cap, p->dtype);
+  const int rc = vocab_validate(p->logits, p->rows, p->V, p->row_stride, p->cap, p->dtype);
   if (rc != XL_OK) return rc;
   if (p->K <= 0 || !vocab_temperature(p->temperature)) return XL_ERR_BAD_SHAPE;
   if (p->K > TOPK_MAX) return XL_ERR_TOO_LARGE;
-  if (p->stats && (reinterpret_cast<uintptr_t>(p->stats) & 7u)) return XL_ERR_BAD_ALIGNMENT;
+  if ((p->stats && (reinterpret_cast<uintptr_t>(p->stats) & 7u)) || (p->dlogits && !vocab_aligned(p->dlogits, p->dtype))) return XL_ERR_BAD_ALIGNMENT;
   if (p->dlogits && p->rows > 1 && p->dlogits_stride < p->V) return XL_ERR_BAD_STRIDE;
   if (p->dlogits) {
     const uintptr_t size = p->dtype == XL_F32 ? 4 : 2, n = (uintptr_t)p->V * size, last = (uintptr_t)(p->rows - 1) * size;

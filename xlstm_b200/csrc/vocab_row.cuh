@@ -281,11 +281,13 @@ static inline bool vocab_bounded(float cap, float temperature) { return cap > 0.
 // temperatures of the entries that compute in fp32
 static inline bool vocab_temperature(float t) { return t >= 1e-4f && t <= 1e6f; }
 // what row-wise entries over logits check in common
-static inline int vocab_validate(int rows, int V, int64_t row_stride, float cap, int dtype) {
+static inline bool vocab_aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == XL_F32 ? 3u : 1u)) == 0; }
+static inline int vocab_validate(const void* logits, int rows, int V, int64_t row_stride, float cap, int dtype) {
   if (dtype != XL_F32 && dtype != XL_BF16) return XL_ERR_BAD_DTYPE;
   if (rows <= 0 || V <= 0 || !(cap == 0.f || (cap >= 1e-6f && cap <= 1e6f))) return XL_ERR_BAD_SHAPE;
   if (rows > 1 && row_stride < V) return XL_ERR_BAD_STRIDE;
   if (V > VOCAB_MAX) return XL_ERR_TOO_LARGE;
+  if (!vocab_aligned(logits, dtype)) return XL_ERR_BAD_ALIGNMENT;   // (whole elements; 16 bytes are not asked for)
   return XL_OK;
 }
 

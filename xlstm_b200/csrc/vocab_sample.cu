@@ -815,7 +815,7 @@ template <typename T> static int vs_launch(const xl_sample_params* p, cudaStream
 extern "C" int xl_softcap_sample(const xl_sample_params* p, void* cuda_stream) {
   using namespace xl;
   if (!p || !p->logits || !p->tokens || !p->u) return XL_ERR_NULL_POINTER;
-  const int rc = vocab_validate(p->rows, p->V, p->row_stride, p->cap, p->dtype);
+  const int rc = vocab_validate(p->logits, p->rows, p->V, p->row_stride, p->cap, p->dtype);
   if (rc != XL_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   return p->dtype == XL_F32 ? vs_launch<float>(p, st) : vs_launch<__nv_bfloat16>(p, st);

@@ -132,7 +132,7 @@ template <typename T> static int tk_choose(const xl_topk_params* p, cudaStream_t
 extern "C" int xl_softcap_topk(const xl_topk_params* p, void* cuda_stream) {
   using namespace xl;
   if (!p || !p->logits || !p->values || !p->ids) return XL_ERR_NULL_POINTER;
-  int rc = vocab_validate(p->rows, p->V, p->row_stride, p->cap, p->dtype);
+  int rc = vocab_validate(p->logits, p->rows, p->V, p->row_stride, p->cap, p->dtype);
   if (rc != XL_OK) return rc;
   if (p->k <= 0 || p->k > p->V || !vocab_temperature(p->temperature)) return XL_ERR_BAD_SHAPE;
   if (p->k > TOPK_MAX) return XL_ERR_TOO_LARGE;
