@@ -335,3 +335,30 @@ def test_captured_draws_do_not_depend_on_the_default_type():
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fails_at", [0, 2])      # in the first warm-up step, in the capture
+def test_a_capture_that_fails_leaves_no_step_behind(fails_at):
+    """The earlier step's buffers are gone by then: it must not be replayed for the settings that it was captured with."""
+    model = _model("cuda")
+    prompt = torch.randint(0, 64, (3, 17), generator=torch.Generator().manual_seed(1)).cuda()
+    gen = lambda: torch.Generator(device="cuda").manual_seed(5)   # noqa: E731
+    a, b = Sampling(0.9, 10), Sampling(1.1)
+    want = model.generate(prompt, 8, sampling=a, generator=gen())[0]
+    assert torch.equal(model.generate(prompt, 8, use_cuda_graph=True, sampling=a, generator=gen())[0], want)
+    forward, calls = model.forward, [0]
+
+    def failing(tokens, *args, **kw):
+        if tokens.shape[1] == 1:
+            calls[0] += 1
+            if calls[0] > fails_at:
+                raise MemoryError
+        return forward(tokens, *args, **kw)
+    model.forward = failing
+    with pytest.raises(MemoryError):
+        model.generate(prompt, 8, use_cuda_graph=True, sampling=b, generator=gen())
+    del model.forward
+    assert model._graph is None
+    assert torch.equal(model.generate(prompt, 8, use_cuda_graph=True, sampling=a, generator=gen())[0], want)
+    model.release_graph()

@@ -503,6 +503,7 @@ class LargeModel:
         dev = self.device
         if self.tp_world > 1:
             self.enable_peer_reduce(max(batch, 256))   # (keeps NCCL where symmetric memory is not available)
+        self._graph = None   # (it belongs to the buffers that are replaced now, also where the capture below fails)
         self._g_state = {i: tuple(t for t in st) for i, st in state.items()}
         self._g_tok = torch.zeros(batch, 1, dtype=torch.long, device=dev)
 
