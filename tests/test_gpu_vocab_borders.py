@@ -127,3 +127,21 @@ def test_rows_beyond_32_bits_are_refused():
             with pytest.raises(XlError, match="capacity"):
                 call()
         del x
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [0.3, 1.0])
+def test_distill_masked_sides_under_a_cap(tag, T):
+    """Under a cap -inf is -cap: a tail, or named tokens, of nothing but -inf have the mass that this says (T = 0.3: down to e^-200 of the rest)."""
+    g = torch.Generator().manual_seed(3)
+    for V in (40, 10007):
+        x = _logits(g, 5, V, DT[tag]).clamp(-20, 20)
+        values, ids, lse = _teacher(g, x, 6, 30.0, T, True, holes=False)
+        named = torch.zeros(5, V, dtype=torch.bool).scatter_(1, ids.long(), True)
+        x[0] = x[0].masked_fill(~named[0], -math.inf)
+        x[1] = x[1].masked_fill(named[1], -math.inf)
+        x[2] = -math.inf
+        x[3] = x[3].masked_fill(~named[3], torch.finfo(DT[tag]).min)
+        x[4] = x[4].masked_fill(~named[4], math.inf)
+        _check_distill(x, values, ids, 30.0, T, lse + 0.1, None)
+        _check_distill(x, values, ids, 30.0, T, None, None)

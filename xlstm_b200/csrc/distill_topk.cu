@@ -211,8 +211,9 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
       xm = block_reduce<WARPS>(xm, OpMax(), s.wf[0]);
       if (blocks > 1) xm = dt_exchange(xm, s.from[2], rank, blocks, OpMax());
       Z.set_ref(fmaxf(xm, xS));
-      mR = xm == -INFINITY ? 0.f : fmaxf(Z(xm), -3e38f);   // (logits of the type's lowest value as masks: z = -inf)
-      mS = xS == -INFINITY ? 0.f : fmaxf(Z(xS), -3e38f);
+      // under a cap -inf is a value like any other; without one it has no mass (and masks of the type's lowest value have z = -inf)
+      mR = CAP ? Z(xm) : xm == -INFINITY ? 0.f : fmaxf(Z(xm), -3e38f);
+      mS = CAP ? Z(xS) : xS == -INFINITY ? 0.f : fmaxf(Z(xS), -3e38f);
     }
   }
   float sS = 0.f;   // of the slice's tokens named
