@@ -145,3 +145,36 @@ def test_distill_masked_sides_under_a_cap(tag, T):
         x[4] = x[4].masked_fill(~named[4], math.inf)
         _check_distill(x, values, ids, 30.0, T, lse + 0.1, None)
         _check_distill(x, values, ids, 30.0, T, None, None)
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+def test_distill_named_tokens_of_the_lowest_value(tag):
+    """Without a cap: the student masks a token (the type's lowest value) that the teacher gives e^-88 / T.  p log q is a number there
+    (6e-39 * 3.4e38 at T = 1), and the loss with it."""
+    import xlstm_b200
+    dt = DT[tag]
+    g = torch.Generator().manual_seed(4)
+    x = _logits(g, 4, 700, dt, 1.0)
+    ids = torch.tensor([[1, 2, 3], [5, 3, 2], [3, 3, 9], [3, 600, 601]], dtype=torch.int32)
+    values = torch.tensor([[0.0, -1.0, -88.0], [1.0, -87.0, 0.0], [-88.0, -89.0, 0.0], [-100.0, 2.0, 1.0]])
+    x[:, 3] = torch.finfo(dt).min
+    for T in (1.0, 0.8, 1.3):
+        keep = (values.double() / T - (values.double() / T).amax(-1, keepdim=True)).amin(-1) > -690.0
+        assert bool(keep.all())
+        for lse in (None, torch.logsumexp(values / T, -1) + 0.2):
+            # (the operator's temperature is a 32-bit number; 1.3 as one is off by 2e-8, and e^(-88 / T) by 68 times that)
+            T32 = float(torch.tensor(T, dtype=torch.float32))
+            want, dz = O.distill(x.double(), values, ids, None, T32, lse), O.distill_grad(x.double(), values, ids, None, T32, lse)
+            assert bool(torch.isfinite(want).all())
+            zmax = float((x.double().masked_fill(x < -1e30, 0.0) / T).abs().max()) + 2.0 / T
+            tol = T * T * (2 * (_rel(zmax) + 64 * E24) + 4 * E24 * zmax) + E24 * want.abs()
+            leaf = x.cuda().requires_grad_()
+            loss = xlstm_b200.distill_topk(leaf, values.cuda(), ids.cuda(), None, T, None if lse is None else lse.cuda())
+            assert ((loss.detach().cpu().double() - want).abs() <= tol).all()
+            loss.sum().backward()
+            grad = xlstm_b200.distill_topk_grad(x.cuda(), values.cuda(), ids.cuda(), None, None, T, None if lse is None else lse.cuda())
+            assert ((grad[0].cpu().double() - want).abs() <= tol).all()   # (other threads, another order of the sums)
+            # (the two launches scale e_k differently, so their last bits differ: each within the gradient's tolerance, q + p + tail <= 3)
+            tol = 3 * T * (2 * _rel(zmax) + 144 * E24) + (torch.finfo(dt).eps / 2 + 2 ** -23) * dz.abs()
+            for got in (grad[1], leaf.grad):
+                assert ((got.cpu().double() - dz).abs() <= tol).all()

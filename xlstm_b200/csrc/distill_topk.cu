@@ -220,12 +220,17 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
   if (warp < with) {
     double E = 0.0, F = 0.0;   // sum of e_k, and of e_k (t_k - z_k)
     for (int k = tid; k < K; k += THREADS) {
-      if (LOSS && !CAP) en.z[k] = Z(en.z[k]);
+      double zk = 0.0;   // z of the student there, without a cap from the logit itself: near the type's lowest value en.z is -inf
+      if (LOSS && CAP) zk = (double)en.z[k] * DT_LN2;
+      if (LOSS && !CAP) {
+        zk = ((double)en.z[k] - (double)Z.ref) * invT;
+        en.z[k] = Z(en.z[k]);
+      }
       double e = 0.0;
       if (en.id[k] >= 0 && live) {
         const double d = en.t[k] - L;
         e = d < -690.0 ? 0.0 : d <= 0.0 ? exp64(d) : exp(d);   // (above 0: a teacher's sum that is not the sum)
-        if (LOSS && !(e == 0.0)) F += e * (en.t[k] - (double)en.z[k] * DT_LN2);
+        if (LOSS && !(e == 0.0)) F += e * (en.t[k] - zk);
       }
       en.e[k] = (float)e;
       E += e;
