@@ -178,3 +178,45 @@ def test_distill_named_tokens_of_the_lowest_value(tag):
             tol = 3 * T * (2 * _rel(zmax) + 144 * E24) + (torch.finfo(dt).eps / 2 + 2 ** -23) * dz.abs()
             for got in (grad[1], leaf.grad):
                 assert ((got.cpu().double() - dz).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("tag", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [40, 10007])
+@pytest.mark.parametrize("T", [1.0, 1.8155349493026733, 4.0, 30.0])
+def test_distill_tails_of_the_lowest_value(tag, V, T):
+    """Without a cap: every token that is not named, or every one that is, is masked by the type's lowest value.  The masked side's own softmax is
+    flat (steps of fp32 there are 2e31), its loss a number wherever 3.4e38 times its share is one."""
+    import xlstm_b200
+    dt = DT[tag]
+    g = torch.Generator().manual_seed(V)
+    x = _logits(g, 5, V, dt, 1.0)
+    ids = torch.stack([torch.randperm(V, generator=g)[:6] for _ in range(5)]).to(torch.int32)
+    values = torch.randn(5, 6, generator=g)
+    named = torch.zeros(5, V, dtype=torch.bool).scatter_(1, ids.long(), True)
+    low = torch.finfo(dt).min
+    x[0] = x[0].masked_fill(~named[0], low)                  # the tail
+    x[1] = x[1].masked_fill(~named[1], low / 2)
+    x[1, (~named[1]).nonzero()[::3, 0]] = low
+    x[2] = x[2].masked_fill(named[2], low)                   # the named ones
+    x[3] = low                                               # everything
+    x[4] = x[4].masked_fill(~named[4], low)
+    ids[4, 2:] = -1                                          # (some of the tail are not masked)
+    T32 = float(torch.tensor(T, dtype=torch.float32))
+    for lse in (None, torch.logsumexp(values / T, -1), torch.logsumexp(values / T, -1) + 0.2):
+        if lse is not None:
+            lse = lse.clamp(min=torch.logsumexp(values.double() / T32, -1) + 1e-6).float()   # (the entries hold a little less than everything)
+        want, dz = O.distill(x.double(), values, ids, None, T32, lse), O.distill_grad(x.double(), values, ids, None, T32, lse)
+        zmax = float((x.double().masked_fill(x < -1e30, 0.0) / T).abs().max()) + 4.0 / T
+        # p are off by 3e-13 of themselves, and a tail of 1 - sum p = 9e-7 (1e-6 and lse's rounding, 1.2e-7) by 4e-7 of itself
+        tol = T * T * (2 * (_rel(zmax) + 64 * E24) + 4 * E24 * zmax) + (4 * E24 + 4e-7) * want.abs()
+        tol_grad = 3 * T * (2 * _rel(zmax) + 144 * E24) + (torch.finfo(dt).eps / 2 + 2 ** -23 + 4e-7) * dz.abs()
+        dev = None if lse is None else lse.cuda()
+        leaf = x.cuda().requires_grad_()
+        loss = xlstm_b200.distill_topk(leaf, values.cuda(), ids.cuda(), None, T, dev)
+        loss.sum().backward()
+        both = xlstm_b200.distill_topk_grad(x.cuda(), values.cuda(), ids.cuda(), None, None, T, dev)
+        for l, d in ((loss.detach(), leaf.grad), both):
+            l, d = l.cpu().double(), d.cpu().double()
+            fits = want.abs() < 3.4e38
+            assert (((l - want).abs() <= tol) | (~fits & (l == math.inf))).all(), (l, want)
+            assert ((d - dz).abs() <= tol_grad).all()

@@ -27,7 +27,8 @@ constexpr int DT_WARPS = 8, DT_BLOCKS = 8;   // warps: at most
 __host__ __device__ constexpr int dt_threads(bool both) { return both ? 256 : 128; }
 constexpr double DT_LN2 = 0.69314718055994530942;
 // what a row leaves for its gradient; ST_FLAGS: 1 if its logits stay below three quarters of the cap, and 2 if a token is named
-// twice; the last two places hold a double
+// twice; the last two places hold a double.  Without a cap ST_LR is what the tail's exponents are relative to, ST_REF what those of
+// the tokens named are, and ST_B has the tail's sum in it.
 enum { ST_LR = 0, ST_L = 1, ST_B = 2, ST_W = 3, ST_FLAGS = 4, ST_REF = 5, ST_TEACHER = 6 };
 
 struct DtShared {
@@ -186,7 +187,10 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     again = (int)st[ST_FLAGS] & 2;
     L = *reinterpret_cast<const double*>(st + ST_TEACHER);
   }
-  float mR = 0.f, mS = 0.f;   // shifts of the two sums: their largest z (with a bounded z: none)
+  // Shifts of the two sums.  Bounded z: none.  Under a cap their largest z.  Without one z may lie anywhere down to the type's
+  // lowest value, where a step of fp32 is 2e31: each sum takes its logits relative to its own largest, refR or refS, from the start,
+  // and the two come together in 64 bits.
+  float mR = 0.f, mS = 0.f, refR = 0.f, refS = 0.f;
   if (LOSS) {
     __syncwarp();
     if (blocks > 1) cluster_wait();
@@ -210,10 +214,16 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
       }
       xm = block_reduce<WARPS>(xm, OpMax(), s.wf[0]);
       if (blocks > 1) xm = dt_exchange(xm, s.from[2], rank, blocks, OpMax());
-      Z.set_ref(fmaxf(xm, xS));
-      // under a cap -inf is a value like any other; without one it has no mass (and masks of the type's lowest value have z = -inf)
-      mR = CAP ? Z(xm) : xm == -INFINITY ? 0.f : fmaxf(Z(xm), -3e38f);
-      mS = CAP ? Z(xS) : xS == -INFINITY ? 0.f : fmaxf(Z(xS), -3e38f);
+      if (CAP) {   // (-inf is a value like any other)
+        mR = Z(xm);
+        mS = Z(xS);
+      } else {
+        Z.set_ref(xm);
+        refR = Z.ref;
+        Z.set_ref(xS);
+        refS = Z.ref;
+        Z.set_ref(fmaxf(xm, xS));
+      }
     }
   }
   float sS = 0.f;   // of the slice's tokens named
@@ -221,9 +231,11 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     double E = 0.0, F = 0.0;   // sum of e_k, and of e_k (t_k - z_k)
     for (int k = tid; k < K; k += THREADS) {
       double zk = 0.0;   // z of the student there, without a cap from the logit itself: near the type's lowest value en.z is -inf
+      float zS = en.z[k] - mS;
       if (LOSS && CAP) zk = (double)en.z[k] * DT_LN2;
       if (LOSS && !CAP) {
         zk = ((double)en.z[k] - (double)Z.ref) * invT;
+        zS = (en.z[k] - refS) * Z.a;
         en.z[k] = Z(en.z[k]);
       }
       double e = 0.0;
@@ -239,7 +251,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
         bool first = o >= slice.first && o < slice.end;
         if (again)   // a token named twice is summed once
           for (int i = 0; i < k; ++i) first = first && en.id[i] != en.id[k];
-        if (first) sS += exp2_approx(en.z[k] - mS);
+        if (first) sS += exp2_approx(zS);
       }
     }
     __syncwarp();
@@ -254,6 +266,8 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
     }
   }
 
+  const float ref = Z.ref;   // of the tokens named
+  if (LOSS && !CAP) Z.ref = refR;
   bool small = true;   // (this thread's, in the second pass: this warp's) logits stay below three quarters of the cap
   if (LOSS) {
     // both sums over the slice.  The first try takes every magnitude for a small one and looks at the largest behind it;
@@ -280,7 +294,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) {
         float z0, z1;
-        f2_unpack(BOUNDED ? z[i] : f2_add(z[i], shift), z0, z1);
+        f2_unpack(BOUNDED || !CAP ? z[i] : f2_add(z[i], shift), z0, z1);
         acc[i & 1] = f2_add(acc[i & 1], f2_pack(exp2_approx(z0), exp2_approx(z1)));
       }
     };
@@ -338,10 +352,18 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
       for (int w = 0; w < with; ++w) { E += s.wd[0][w]; F += s.wd[1][w]; }
       const double left = given && live && !everything ? fmax(0.0, 1.0 - E) : 0.0;   // p_tail
       // sums in one scale, and the four logarithms in four lanes
-      const float top = BOUNDED ? 0.f : sR > 0.f ? (sS > 0.f ? fmaxf(mR, mS) : mR) : mS;
+      double oR = (double)mR, oS = (double)mS;   // (without a cap the larger one is 0)
+      if (!CAP) {
+        const double scale = invT * 1.4426950408889634;
+        oR = ((double)refR - (double)ref) * scale;
+        oS = ((double)refS - (double)ref) * scale;
+        mR = (float)oR;
+        mS = (float)oS;
+      }
+      const float top = BOUNDED || !CAP ? 0.f : sR > 0.f ? (sS > 0.f ? fmaxf(mR, mS) : mR) : mS;
       const double tR = BOUNDED || sR == 0.f ? sR : sR * exp2_approx(mR - top), tS = BOUNDED || sS == 0.f ? sS : sS * exp2_approx(mS - top);
       const double lg = log2_64(lane == 0 ? (double)sR : lane == 1 ? tR + tS : lane == 2 ? E : left);
-      const double lR = __shfl_sync(0xffffffffu, lg, 0) + (double)mR, l = __shfl_sync(0xffffffffu, lg, 1) + (double)top;   // log2(0) = -inf
+      const double lR = __shfl_sync(0xffffffffu, lg, 0) + oR, l = __shfl_sync(0xffffffffu, lg, 1) + (double)top;   // log2(0) = -inf
       const double lE = __shfl_sync(0xffffffffu, lg, 2), lleft = __shfl_sync(0xffffffffu, lg, 3);
       if (lane == 0) {
         double loss = 0.0, W = 0.0;
@@ -351,15 +373,16 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
           loss = given ? F + E * (l * DT_LN2 - L) : F * iE + (l - lE) * DT_LN2 - L;
           if (!(left == 0.0)) loss += left * (lleft - lR + l) * DT_LN2;
         }
-        s.lR = sR == 0.f ? 0.f : (float)lR;
+        s.lR = !CAP ? refR : sR == 0.f ? 0.f : (float)lR;
         s.l = (float)l;
         s.B = sR == 0.f ? 0.f : (float)(W * (double)((float)tR / (float)(tR + tS)) - left);
+        if (!CAP && sR != 0.f) s.B /= sR;
         s.W = (float)W;
         s.pscale = given ? 1.f : (float)iE;
         if (rank == 0) {
           p.loss[row] = (float)((double)p.temperature * (double)p.temperature * loss);
           if (st) {
-            st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W; st[ST_FLAGS] = (all_small ? 1.f : 0.f) + (float)named_twice; st[ST_REF] = Z.ref;
+            st[ST_LR] = s.lR; st[ST_L] = s.l; st[ST_B] = s.B; st[ST_W] = s.W; st[ST_FLAGS] = (all_small ? 1.f : 0.f) + (float)named_twice; st[ST_REF] = ref;
             *reinterpret_cast<double*>(st + ST_TEACHER) = given ? L : L + lE * DT_LN2;
           }
         }
@@ -374,7 +397,8 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
 
   T* dx = static_cast<T*>(p.dlogits) + row * p.dlogits_stride;
   const bool wide = (reinterpret_cast<uintptr_t>(dx + slice.head) & 15u) == 0;   // the gradient's vectors lie like the logits'
-  const float g = live ? (p.weight ? p.weight[row * p.weight_stride] : 1.f) * p.temperature : 0.f, gB = g * s.B, lR = s.lR;
+  const float g = live ? (p.weight ? p.weight[row * p.weight_stride] : 1.f) * p.temperature : 0.f, gB = g * s.B, lR = CAP ? s.lR : 0.f;
+  if (!CAP) Z.ref = s.lR;
   const float bend = CAP ? gB * Z.flat : 0.f;   // slope 1 - tanh^2 = 1 - (z / a)^2
   const f32x2 gB2 = f2_dup(gB), bend2 = f2_dup(-bend), shift = f2_dup(-lR);
   auto store = [&](const uint4& out, int v) {
@@ -391,7 +415,7 @@ __global__ void __launch_bounds__(dt_threads(LOSS && GRAD), LOSS && GRAD ? 4 : 8
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
       float e0, e1;
-      f2_unpack(f2_add(z[i], shift), e0, e1);
+      f2_unpack(CAP ? f2_add(z[i], shift) : z[i], e0, e1);
       const f32x2 e = f2_pack(exp2_approx(e0), exp2_approx(e1));
       d[i] = f2_mul(e, CAP ? f2_fma(f2_mul(z[i], z[i]), bend2, gB2) : gB2);
     }
